@@ -44,6 +44,8 @@ enum : int {
   kWhereMisc = 6,
   kWhereGemm = 7,
   kWhereExchange = 8,  // a peer's flag did not arrive in time (info0 = source rank)
+  kWhereCache = 9,     // page copies and cache compaction
+  kWhereScore = 10,    // token log probabilities
 };
 
 __device__ __forceinline__ void report_status(TmcDeviceStatus *s, int code, int where,

@@ -1,0 +1,452 @@
+// Token log probabilities, entropy, rank and top alternatives (logprobs.cuh).
+//
+// For a row x of V logits and m = max x, with
+//   s = sum e^(x - m),  u = sum e^(x - m) (x - m)
+// the log normaliser is m + log s, the target's log probability
+// (x_t - m) - log s and the entropy log s - u / s. One pass over the row keeps
+// (m, s, u) per thread, rescaled when the running maximum rises, and counts
+// the logits that come before the target (larger, or equal at a lower index).
+// u is summed about the maximum so that a peaked row's small entropy does not
+// come out as a difference of two large numbers.
+//
+// The top alternatives come from the same read: every thread keeps its largest
+// logit as an ordered (value, index) key; the top-th largest of these keys is a
+// lower bound for the row's top-th logit, so only the at most `top` threads
+// whose own largest reaches it are read again, each by a whole warp (from L2).
+//
+// A row is shared by a thread-block cluster when there are few rows; its CTAs
+// hand their (m, s, u), counts and top lists to the cluster's first CTA
+// through distributed shared memory.
+#include "logprobs.cuh"
+
+#include <cuda_bf16.h>
+
+#include "mbarrier.cuh"
+
+namespace tmc {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+using Key = unsigned long long;
+
+template <typename T>
+struct Logit;
+template <>
+struct Logit<float> {
+  static constexpr int kVec = 4;  // elements of a 16-byte vector
+  static __device__ __forceinline__ float get(const float *p) { return *p; }
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x);
+    x[1] = __uint_as_float(v.y);
+    x[2] = __uint_as_float(v.z);
+    x[3] = __uint_as_float(v.w);
+  }
+};
+template <>
+struct Logit<__half> {
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = half2_bits_to_float2(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+};
+template <>
+struct Logit<__nv_bfloat16> {
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+// Running (maximum, sum e^(x-m), sum e^(x-m) (x-m)) of a softmax.
+struct Stats {
+  float m, s, u;
+};
+__device__ __forceinline__ Stats empty_stats() { return {-INFINITY, 0.0f, 0.0f}; }
+
+// The statistics of two disjoint parts together. A part without finite weight
+// (m = -inf: nothing but masked logits) leaves the other as it is.
+__device__ __forceinline__ Stats join(const Stats &a, const Stats &b) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return {m, a.s + b.s, a.u + b.u};
+  const float da = fmaxf(a.m - m, -1e30f), db = fmaxf(b.m - m, -1e30f);
+  const float fa = exp2f(da * kLog2e), fb = exp2f(db * kLog2e);
+  return {m, fmaf(a.s, fa, b.s * fb), fmaf(fmaf(a.s, da, a.u), fa, fmaf(b.s, db, b.u) * fb)};
+}
+
+__device__ __forceinline__ Stats warp_join(Stats a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
+                 __shfl_xor_sync(0xffffffffu, a.u, o)});
+  return a;
+}
+
+// N logits (index of the first: at) into the running statistics, the count
+// before the target and the thread's largest key.
+template <int N, bool TOP>
+__device__ __forceinline__ void take(const float (&x)[N], int at, float xt, int target, Stats &st, int &before,
+                                     float &best, int &best_at) {
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+  if (mx > st.m) {
+    if (st.m != -INFINITY) {
+      const float d = fmaxf(st.m - mx, -1e30f), f = exp2f(d * kLog2e);
+      st.u = fmaf(st.s, d, st.u) * f;
+      st.s *= f;
+    }
+    st.m = mx;
+    if (TOP) {
+      best = mx;
+      best_at = at;
+    }
+  }
+  const float m = st.m == -INFINITY ? 0.0f : st.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] - m;
+    const float e = exp2f(d * kLog2e);
+    st.s += e;
+    st.u = fmaf(e, fmaxf(d, -1e30f), st.u);  // a masked logit: 0 times a finite number
+    before += (x[i] > xt || (x[i] == xt && at + i < target)) ? 1 : 0;
+  }
+}
+
+// Larger logits first, then lower indices; NaN counts as -inf, -0 as 0.
+__device__ __forceinline__ Key order_key(float x, int index) { return argmax_key(__fadd_rn(x, 0.0f), index); }
+
+__device__ __forceinline__ Key shfl_key(Key k, int lane) { return __shfl_sync(0xffffffffu, k, lane); }
+// Descending bitonic sort of one key per lane.
+__device__ __forceinline__ Key warp_sort(Key k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      const Key o = __shfl_xor_sync(0xffffffffu, k, step);
+      const bool first = (lane & step) == 0, descending = (lane & size) == 0;
+      k = (first == descending) ? (k > o ? k : o) : (k < o ? k : o);
+    }
+  }
+  return k;
+}
+// The 32 largest of two descending lists of 32 (one key of each per lane), descending.
+__device__ __forceinline__ Key warp_merge(Key a, Key b, int lane) {
+  const Key r = shfl_key(b, 31 - lane);
+  Key k = a > r ? a : r;
+#pragma unroll
+  for (int step = 16; step > 0; step >>= 1) {
+    const Key o = __shfl_xor_sync(0xffffffffu, k, step);
+    k = (lane & step) == 0 ? (k > o ? k : o) : (k < o ? k : o);
+  }
+  return k;
+}
+
+// Warp 0 merges `lists` descending lists of 32 keys in shared memory; every
+// warp's list has been written.
+__device__ __forceinline__ Key merge_lists(const Key *lists, int n, int lane) {
+  Key k = lists[lane];
+  for (int i = 1; i < n; ++i) k = warp_merge(k, lists[i * 32 + lane], lane);
+  return k;
+}
+
+// What a CTA hands to the cluster's first CTA.
+struct Part {
+  Stats st;
+  int before;
+  Key top[32];
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The address of a shared variable in the cluster's first CTA, and stores to it.
+__device__ __forceinline__ uint32_t in_first_cta(const void *local) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(local)));
+  return r;
+}
+__device__ __forceinline__ void store_cluster(uint32_t at, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t at, Key v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+
+// Grid (rows x cluster); the CTAs of a cluster share one row.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobsParams p) {
+  using L = Logit<T>;
+  constexpr int N = L::kVec;
+  __shared__ Stats warp_stats[kWarps];
+  __shared__ int warp_before[kWarps];
+  __shared__ Key lists[kWarps * 32];
+  __shared__ Key threshold;
+  __shared__ int flagged[kLogprobsMaxTop];
+  __shared__ int flagged_count;
+  __shared__ Part parts[kMaxCluster];
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int csize = (int)cluster_size(), crank = (int)cluster_rank(), row = blockIdx.x / csize;
+  cluster_arrive();  // waited for before the first store to another CTA's memory
+  const T *x = static_cast<const T *>(p.logits) + (long long)row * p.row_stride;
+
+  const int target = p.targets != nullptr ? p.targets[row] : -1;
+  const bool bad_target = target < -1 || target >= p.vocab;
+  if (bad_target && tid == 0 && crank == 0) report_status(p.status, kStatusTokenRange, kWhereScore, target, row);
+  const bool given = target >= 0 && !bad_target;
+  const float xt = given ? L::get(x + target) : INFINITY;
+
+  // This CTA's logits [begin, end): whole vectors but for the row's ends. The
+  // first `head` logits of the row come before its first 16-byte boundary.
+  const int misaligned = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int head = min(misaligned ? N - misaligned : 0, p.vocab);
+  const int vectors = (p.vocab - head) / N, tail = (p.vocab - head) % N;
+  const int per = (vectors + csize - 1) / csize;
+  const int v0 = min(vectors, crank * per), v1 = min(vectors, v0 + per);
+  const uint4 *body = reinterpret_cast<const uint4 *>(x + head);
+
+  Stats st = empty_stats();
+  int before = 0;
+  float best = -INFINITY;
+  int best_at = -1;  // first index of the vector that holds the thread's largest logit
+  if (crank == 0 && tid < head) {
+    const float one[1] = {L::get(x + tid)};
+    take<1, TOP>(one, tid, xt, target, st, before, best, best_at);
+  }
+  constexpr int kUnroll = 4;
+  for (int v = v0 + tid; v < v1; v += kThreads * kUnroll) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (v + i * kThreads < v1) raw[i] = __ldg(body + v + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (v + i * kThreads < v1) {
+        float f[N];
+        L::unpack(raw[i], f);
+        take<N, TOP>(f, head + (v + i * kThreads) * N, xt, target, st, before, best, best_at);
+      }
+  }
+  if (crank == csize - 1 && tid < tail) {
+    const int at = head + vectors * N + tid;
+    const float one[1] = {L::get(x + at)};
+    take<1, TOP>(one, at, xt, target, st, before, best, best_at);
+  }
+
+  // The CTA's statistics.
+  {
+    const Stats w = warp_join(st);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (lane == 0) {
+      warp_stats[warp] = w;
+      warp_before[warp] = before;
+    }
+  }
+
+  Key top_key = 0;  // warp 0, lane i: the CTA's i-th largest (0: none)
+  if (TOP) {
+    // Keys order by value, then by the lower index. A thread's own largest
+    // element is looked for again in the vector that held it.
+    Key mine = 0;
+    if (best_at >= 0) {
+      mine = order_key(best, best_at);
+      if (best_at >= head && best_at < head + vectors * N) {
+        for (int i = 0; i < N; ++i)
+          if (L::get(x + best_at + i) == best) {
+            mine = order_key(best, best_at + i);
+            break;
+          }
+      }
+    }
+    // The top-th largest of the threads' largest keys bounds the CTA's top-th
+    // key from below. Threads that saw only -inf or NaN have no key: their
+    // elements count when there are too few others.
+    lists[warp * 32 + lane] = warp_sort(mine, lane);
+    if (tid == 0) flagged_count = 0;
+    __syncthreads();
+    if (warp == 0) {
+      const Key k = merge_lists(lists, kWarps, lane);
+      if (lane == p.top - 1) threshold = k;
+    }
+    __syncthreads();
+    const Key bound = threshold;
+    Key list = 0;  // this warp's descending list, one key per lane
+    auto offer = [&](Key k) {
+      // Lanes whose key reaches the bound and the full list insert them one
+      // after another.
+      const Key last = shfl_key(list, 31);
+      unsigned want = __ballot_sync(0xffffffffu, k >= bound && k > last);
+      while (want) {
+        const Key c = shfl_key(k, __ffs(want) - 1);
+        want &= want - 1;
+        const int at = __popc(__ballot_sync(0xffffffffu, list > c));
+        const Key up = __shfl_up_sync(0xffffffffu, list, 1);
+        list = lane < at ? list : (lane == at ? c : up);
+      }
+    };
+    if (bound != 0) {
+      if (mine >= bound) flagged[atomicAdd(&flagged_count, 1)] = tid;
+      __syncthreads();
+      const int n = flagged_count;
+      for (int f = warp; f < n; f += kWarps) {
+        const int t = flagged[f];
+        // thread t's elements, spread over the lanes
+        const int mine_vectors = v1 - v0 > t ? (v1 - v0 - t + kThreads - 1) / kThreads : 0;
+        for (int e0 = 0; e0 < mine_vectors * N; e0 += 32) {
+          const int e = e0 + lane;
+          Key k = 0;
+          if (e < mine_vectors * N) {
+            const int at = head + (v0 + t + e / N * kThreads) * N + e % N;
+            k = order_key(L::get(x + at), at);
+          }
+          offer(k);
+        }
+        Key k = 0;
+        if (lane == 0 && crank == 0 && t < head) k = order_key(L::get(x + t), t);
+        if (lane == 1 && crank == csize - 1 && t < tail) {
+          const int at = head + vectors * N + t;
+          k = order_key(L::get(x + at), at);
+        }
+        offer(k);
+      }
+    } else {
+      // Fewer than `top` threads saw a logit above -inf (a short or masked
+      // row): every element is offered.
+      __syncthreads();
+      const int e1 = (v1 - v0) * N;
+      for (int e0 = warp * 32; e0 < e1; e0 += kThreads) {
+        const int at = head + v0 * N + e0 + lane;
+        offer(e0 + lane < e1 ? order_key(L::get(x + at), at) : 0ull);
+      }
+      Key k = 0;
+      if (warp == 0 && crank == 0 && lane < head) k = order_key(L::get(x + lane), lane);
+      offer(k);
+      k = 0;
+      if (warp == 0 && crank == csize - 1 && lane < tail) {
+        const int at = head + vectors * N + lane;
+        k = order_key(L::get(x + at), at);
+      }
+      offer(k);
+    }
+    lists[warp * 32 + lane] = list;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    if (TOP) top_key = merge_lists(lists, kWarps, lane);
+    Stats all = lane < kWarps ? warp_stats[lane] : empty_stats();
+    all = warp_join(all);
+    int n = lane < kWarps ? warp_before[lane] : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    st = all;
+    before = n;
+  }
+  cluster_wait();
+  if (csize > 1) {
+    if (warp == 0) {
+      Part *part = parts + crank;
+      if (lane == 0) {
+        store_cluster(in_first_cta(&part->st.m), __float_as_uint(st.m));
+        store_cluster(in_first_cta(&part->st.s), __float_as_uint(st.s));
+        store_cluster(in_first_cta(&part->st.u), __float_as_uint(st.u));
+        store_cluster(in_first_cta(&part->before), (uint32_t)before);
+      }
+      if (TOP) store_cluster(in_first_cta(&part->top[lane]), top_key);
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (crank != 0) return;
+    if (warp == 0) {
+      st = lane < csize ? parts[lane].st : empty_stats();
+      st = warp_join(st);
+      before = lane < csize ? parts[lane].before : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      if (TOP)
+        for (int c = 1; c < csize; ++c) top_key = warp_merge(top_key, parts[c].top[lane], lane);
+    }
+  }
+  if (warp != 0) return;
+  // With nothing but masked logits no token has any probability: every log
+  // probability is -inf, the entropy 0. +inf or NaN among the logits make s,
+  // and with it every result, NaN.
+  const bool none = st.m == -INFINITY && st.s == 0.0f;
+  const float log_s = none ? 0.0f : log2f(st.s) * kLn2;
+  auto log_p = [&](float v) { return none ? -INFINITY : (v - st.m) - log_s; };
+  if (lane == 0) {
+    if (p.logprobs) p.logprobs[row] = bad_target ? NAN : (given ? log_p(xt) : 0.0f);
+    if (p.entropy) p.entropy[row] = none ? 0.0f : log_s - st.u / st.s;
+    if (p.ranks) p.ranks[row] = given ? before : -1;
+  }
+  if (TOP && lane < p.top) {
+    const int id = argmax_key_index(top_key);
+    p.top_ids[(size_t)row * p.top + lane] = id;
+    p.top_logprobs[(size_t)row * p.top + lane] = log_p(L::get(x + id));
+  }
+}
+
+template <typename T>
+cudaError_t launch(const LogprobsParams &p, int cluster, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cluster * p.rows);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return p.top > 0 ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, p)
+                   : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, p);
+}
+
+}  // namespace
+
+cudaError_t launch_token_logprobs(const LogprobsParams &p, int type, int num_sms, cudaStream_t stream) {
+  if (p.rows < 0 || p.rows > 0x7fffffff / kMaxCluster || p.vocab <= 0 || p.top < 0 || p.top > kLogprobsMaxTop || p.top > p.vocab ||
+      p.row_stride < p.vocab)
+    return cudaErrorInvalidValue;
+  if (p.rows == 0) return cudaSuccess;
+  // CTAs per row: enough to fill the GPU, each with some thousand logits.
+  int cluster = 1;
+  while (cluster < kMaxCluster && p.rows * cluster < 2 * num_sms && p.vocab / cluster > 4096) cluster *= 2;
+  switch (type) {
+    case kLogitsF16: return launch<__half>(p, cluster, stream);
+    case kLogitsF32: return launch<float>(p, cluster, stream);
+    case kLogitsBF16: return launch<__nv_bfloat16>(p, cluster, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace tmc

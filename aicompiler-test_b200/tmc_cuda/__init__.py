@@ -106,6 +106,14 @@ _sig("tmc_k_paged_attention_f16_ex", c_int, c_void_p, c_void_p, c_void_p, c_void
      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
      c_void_p, c_int, c_int, c_void_p, c_void_p)
 _sig("tmc_k_fill_normal_f16", c_int, c_void_p, c_size_t, c_uint64, c_float, c_float, c_void_p)
+_sig("tmc_k_window_attention_workspace_bytes", c_size_t, *[c_int] * 7)
+_sig("tmc_k_window_attention", c_int, c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_int,
+     c_void_p, c_int, c_void_p, c_void_p, c_void_p, *[c_int] * 11, c_float, c_void_p, c_size_t, c_void_p, c_void_p)
+_sig("tmc_k_token_logprobs", c_int, c_void_p, c_int, ctypes.c_int64, c_void_p, c_int, c_int, c_void_p, c_void_p,
+     c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p)
+_sig("tmc_k_kv_copy_pages", c_int, c_void_p, c_int, c_int, c_size_t, c_void_p, c_void_p, c_int, c_void_p, c_void_p)
+_sig("tmc_k_kv_compact", c_int, c_void_p, *[c_int] * 6, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int,
+     c_void_p, c_void_p, c_int, c_void_p, c_void_p)
 
 
 def last_error() -> str:
@@ -399,6 +407,76 @@ def paged_attention_f16(rt: Runtime, q: Buffer, out: Buffer, k_pool: Buffer, v_p
         positions.ptr, rows, hq, hkv, d, page_size, pool_pages, capacity, max_splits, min_chunk,
         workspace.ptr if workspace is not None else None, counters.ptr, schedule, row_group, rt.status_ptr,
         rt.stream))
+
+
+# Serving-cache kernels: arrays are Buffers or objects with data_ptr() and dtype
+# (tensors of another library); `stream` is a cudaStream_t value, the runtime's
+# stream when None.
+
+_DTYPE_NAMES = {"float16": F16, "float32": F32, "bfloat16": BF16}
+
+
+def _ptr(array):
+    if array is None:
+        return None
+    return array.ptr if isinstance(array, Buffer) else array.data_ptr()
+
+
+def _dtype_of(array) -> int:
+    return array.dtype if isinstance(array, Buffer) else _DTYPE_NAMES[str(array.dtype).rpartition(".")[2]]
+
+
+def _nbytes(array) -> int:
+    if isinstance(array, Buffer):
+        return array.count * (4 if array.dtype in (F32, I32) else 2)
+    return array.numel() * array.element_size()
+
+
+def window_attention_workspace_bytes(sequences: int, max_rows: int, hq: int, hkv: int, d: int, window: int,
+                                     sinks: int = 0) -> int:
+    return int(lib.tmc_k_window_attention_workspace_bytes(sequences, max_rows, hq, hkv, d, window, sinks))
+
+
+def window_attention(rt: Runtime, q, out, k_pool, v_pool, block_table, table_stride: int, table_rows, row_starts,
+                     first_positions, sequences: int, rows: int, max_rows: int, hq: int, hkv: int, d: int,
+                     page_size: int, pool_pages: int, capacity: int, window: int, sinks: int = 0, scale: float = 0.0,
+                     q_stride: int | None = None, out_stride: int | None = None, workspace=None, stream=None):
+    """Attention over the paged cache with a sliding window and `sinks` first positions that
+    stay visible, for ragged query rows (tmc_k_window_attention); fp16 or bf16, as q."""
+    check(lib.tmc_k_window_attention(
+        _ptr(q), hq * d if q_stride is None else q_stride, _ptr(out), hq * d if out_stride is None else out_stride,
+        _ptr(k_pool), _ptr(v_pool), _dtype_of(q), _ptr(block_table), table_stride, _ptr(table_rows), _ptr(row_starts),
+        _ptr(first_positions), sequences, rows, max_rows, hq, hkv, d, page_size, pool_pages, capacity, window, sinks,
+        scale, _ptr(workspace), 0 if workspace is None else _nbytes(workspace), rt.status_ptr,
+        rt.stream if stream is None else stream))
+
+
+def token_logprobs(rt: Runtime, logits, targets, rows: int, vocab: int, logprobs, entropy=None, ranks=None,
+                   top: int = 0, top_ids=None, top_logprobs=None, row_stride: int | None = None, stream=None):
+    """Log probability, rank and entropy of one given token per row of logits, with the `top`
+    largest alternatives (tmc_k_token_logprobs)."""
+    check(lib.tmc_k_token_logprobs(
+        _ptr(logits), _dtype_of(logits), vocab if row_stride is None else row_stride, _ptr(targets), rows, vocab,
+        _ptr(logprobs), _ptr(entropy), _ptr(ranks), top, _ptr(top_ids) if top else None,
+        _ptr(top_logprobs) if top else None, rt.status_ptr, rt.stream if stream is None else stream))
+
+
+def kv_copy_pages(rt: Runtime, pools, pool_count: int, pool_pages: int, page_bytes: int, src, dst, count: int,
+                  stream=None):
+    """Copy page src[i] to page dst[i] of every pool; pools: device array of addresses
+    (tmc_k_kv_copy_pages)."""
+    check(lib.tmc_k_kv_copy_pages(_ptr(pools), pool_count, pool_pages, page_bytes, _ptr(src), _ptr(dst), count,
+                                  rt.status_ptr, rt.stream if stream is None else stream))
+
+
+def kv_compact(rt: Runtime, pools, layers: int, pool_pages: int, hkv: int, d: int, page_size: int, src_pages,
+               src_count: int, dst_pages, dst_count: int, keep, count: int, first: int = 0, rope_cos=None,
+               rope_sin=None, rope_rows: int = 0, dtype: int = F16, stream=None):
+    """Move the kept rows of a sequence together into other pages, keys turned by the distance
+    moved (tmc_k_kv_compact)."""
+    check(lib.tmc_k_kv_compact(_ptr(pools), layers, dtype, pool_pages, hkv, d, page_size, _ptr(src_pages), src_count,
+                               _ptr(dst_pages), dst_count, _ptr(keep), count, first, _ptr(rope_cos), _ptr(rope_sin),
+                               rope_rows, rt.status_ptr, rt.stream if stream is None else stream))
 
 
 def fill_normal_f16(rt: Runtime, buf: Buffer, seed: int, mean: float, std: float):

@@ -273,6 +273,84 @@ int tmc_k_paged_attention_f16_noalloc(const void *q, void *out, const void *k_po
                                       int page_size, int pool_pages, int capacity, int max_splits,
                                       int min_chunk, void *status, void *stream);
 
+/* ---- serving-cache kernels -------------------------------------------------
+ * Attention with a sliding window, scores of answered tokens, and copies inside
+ * the cache. No counterpart in the reference. They run on the device that holds
+ * `out` (attention), `logits` (scores) or `pools` (copies), whatever device is
+ * current; `stream` belongs to that device. All can be captured into a graph.
+ * Failures seen on the GPU (a missing page, an index out of range) go to
+ * `status` (tmc_runtime_status_ptr() or NULL) and skip what they concern. */
+
+/* Causal attention over the paged cache for ragged query rows, with a sliding
+ * window and first positions that stay visible: the query at position p sees
+ * the keys j <= p with p - j < window or j < sinks (window >= capacity: all
+ * earlier keys).
+ *   q, out   rows of [hq, d], q_stride / out_stride elements from row to row
+ *            (multiples of 8, at least hq * d), fp16 or bf16 (dtype)
+ *   k_pool,
+ *   v_pool   [pool_pages, hkv, page_size, d], any page_size >= 1, same dtype
+ *   block_table [.., table_stride] int32, row table_rows[s] for sequence s;
+ *            only pages that hold a visible key are looked at
+ *   row_starts [sequences + 1] int32: sequence s owns the query rows
+ *            row_starts[s] .. row_starts[s + 1] - 1 (none is allowed), at the
+ *            positions first_positions[s], first_positions[s] + 1, ..
+ *            (below capacity); rows of no sequence are left as they were
+ *   rows     rows of q and out; max_rows: the most rows of one sequence (1:
+ *            single-token decoding)
+ * hq a multiple of hkv, d in {16, 32, 64, 128}, scale 0 for 1 / sqrt(d);
+ * pointers 16-byte aligned. A row all of whose pages are missing becomes 0.
+ * workspace: with tmc_k_window_attention_workspace_bytes(...) bytes a launch of
+ * few rows over a wide window is split further; with fewer, or NULL, it is
+ * split less and takes longer. Its contents need not be set, and nothing in it
+ * outlasts the call; calls that overlap on the GPU need one each. */
+size_t tmc_k_window_attention_workspace_bytes(int sequences, int max_rows, int hq, int hkv, int d, int window,
+                                              int sinks);
+int tmc_k_window_attention(const void *q, int64_t q_stride, void *out, int64_t out_stride, const void *k_pool,
+                           const void *v_pool, int dtype, const int32_t *block_table, int table_stride,
+                           const int32_t *table_rows, const int32_t *row_starts, const int32_t *first_positions,
+                           int sequences, int rows, int max_rows, int hq, int hkv, int d, int page_size,
+                           int pool_pages, int capacity, int window, int sinks, float scale, void *workspace,
+                           size_t workspace_bytes, void *status, void *stream);
+
+/* Scores of one token per row of logits (fp16, bf16 or fp32; the first `vocab`
+ * of each row, row_stride >= vocab elements apart, aligned to their element):
+ *   logprobs [rows]  log softmax(row)[targets[row]]
+ *   entropy  [rows]  -sum p log p, natural logarithms
+ *   ranks    [rows]  logits before the target: larger, or equal at a lower index
+ *   top_ids, top_logprobs [rows, top]  the `top` largest logits in that order
+ * top <= 32. Each result but the pair of top arrays may be NULL (targets too,
+ * without logprobs and ranks). A target of -1 is none: log probability 0, rank
+ * -1; another one outside [0, vocab) is reported, with NaN and rank -1. A logit
+ * of -inf is a masked token; a row of nothing else has log probabilities -inf
+ * and entropy 0. +inf or NaN in a row make its log probabilities and entropy
+ * NaN (NaN ranks as -inf). */
+int tmc_k_token_logprobs(const void *logits, int dtype, int64_t row_stride, const int32_t *targets, int rows, int vocab,
+                         float *logprobs, float *entropy, int32_t *ranks, int top, int32_t *top_ids,
+                         float *top_logprobs, void *status, void *stream);
+
+/* Copy page src[i] to page dst[i] in every pool (forking a sequence, moving
+ * pages). pools: device array of pool_count pool addresses (16-byte aligned),
+ * each pool_pages pages of page_bytes bytes (a multiple of 16); src, dst:
+ * device arrays of `count` pages. Sources may repeat; targets are distinct and
+ * none is the source of another pair. */
+int tmc_k_kv_copy_pages(void *const *pools, int pool_count, int pool_pages, size_t page_bytes, const int32_t *src,
+                        const int32_t *dst, int count, void *status, void *stream);
+
+/* Move the kept rows of a sequence together: position keep[i] of the pages
+ * src_pages[0 .. src_count) becomes position first + i of the pages
+ * dst_pages[0 .. dst_count), in every layer and KV head. Values move as they
+ * are; keys, stored rotated by their position (interleaved pairs, as the
+ * decoder's RoPE), are turned by the distance moved, in fp32, with row
+ * |keep[i] - first - i| of rope_cos / rope_sin [rope_rows, d / 2], and rounded
+ * once. Without tables keys move as they are. pools: device array of 2 * layers
+ * pool addresses (K, V of layer 0, K, V of layer 1, ..), 16-byte aligned,
+ * [pool_pages, hkv, page_size, d] fp16 or bf16; d % 8 == 0. No page of
+ * dst_pages is one of src_pages. */
+int tmc_k_kv_compact(void *const *pools, int layers, int dtype, int pool_pages, int hkv, int d, int page_size,
+                     const int32_t *src_pages, int src_count, const int32_t *dst_pages, int dst_count,
+                     const int32_t *keep, int count, int first, const float *rope_cos, const float *rope_sin,
+                     int rope_rows, void *status, void *stream);
+
 /* Deterministic N(0, std^2) fp16 fill from a counter-based hash generator
  * (synthetic random-init weights without a host round trip). */
 int tmc_k_fill_normal_f16(void *dst, size_t count, uint64_t seed, float mean, float stddev,
