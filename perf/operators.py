@@ -325,7 +325,10 @@ def _own_attention(c, st):
     tmc, rt = _library()
     need = tmc.window_attention_workspace_bytes(c["seqs"], st["most_rows"], c["hq"], c["hkv"], c["d"], c["window"],
                                                 c["sinks"])
-    tmc.window_attention(rt, st["q"], st["out"], st["k"], st["v"], st["table"], st["stride"], st["table_rows"],
+    # Table rows shorter than their sequence name the pool's last page (-1, as an index), by its own
+    # number here; the table of a single sequence is whole.
+    table = st["table"] if c["seqs"] == 1 else st["table"].remainder(st["pool_pages"])
+    tmc.window_attention(rt, st["q"], st["out"], st["k"], st["v"], table, st["stride"], st["table_rows"],
                          st["starts"], st["first"], c["seqs"], st["total"], st["most_rows"], c["hq"], c["hkv"], c["d"],
                          c["page"], st["pool_pages"], c["context"], c["window"], c["sinks"],
                          workspace=_workspace(need), stream=_stream())
