@@ -19,8 +19,9 @@
 
 #include <cuda_bf16.h>
 
+#include <map>
 #include <mutex>
-#include <unordered_map>
+#include <utility>
 
 #include "mbarrier.cuh"
 
@@ -28,7 +29,8 @@ namespace tmc {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxCluster = 16;  // CTAs of a decode cluster (8 where 16 are not available)
+constexpr int kMaxCluster = 8;    // CTAs of a decode cluster
+constexpr int kDecodePerSm = 3;  // decode CTAs that an SM holds
 constexpr int kMaxOuter = 32;    // splits that meet through the workspace
 
 // ---- element types ------------------------------------------------------------------
@@ -151,16 +153,26 @@ __device__ __forceinline__ Visible visible_keys(const WindowAttentionParams &p, 
   return v;
 }
 
-// The pool row (of D elements) of key j for KV head h; -1 when its page is missing.
-__device__ __forceinline__ long long pool_row(const WindowAttentionParams &p, const int *table, int j, int h, int s) {
-  const int logical = j / p.page_size;
-  const int page = logical < p.table_stride ? table[logical] : -1;
-  if (page < 0 || page >= p.pool_pages) {
-    report_status(p.status, page < 0 ? kStatusPageMissing : kStatusPageRange, kWhereAttention,
-                  page < 0 ? logical : page, s);
+// Where key j of a sequence is: its table entry (as loaded, unchecked: -1
+// beyond the table) and its place in the page.
+struct KeyPlace {
+  int logical, page, offset;
+};
+__device__ __forceinline__ KeyPlace find_key(const WindowAttentionParams &p, const int *table, int j) {
+  KeyPlace k;
+  k.logical = p.page_shift >= 0 ? j >> p.page_shift : j / p.page_size;
+  k.offset = j - k.logical * p.page_size;
+  k.page = k.logical < p.table_stride ? table[k.logical] : -1;
+  return k;
+}
+// The key's pool row (of D elements) for KV head h; -1, reported, when its page is missing.
+__device__ __forceinline__ long long pool_row(const WindowAttentionParams &p, const KeyPlace &k, int h, int s) {
+  if (k.page < 0 || k.page >= p.pool_pages) {
+    report_status(p.status, k.page < 0 ? kStatusPageMissing : kStatusPageRange, kWhereAttention,
+                  k.page < 0 ? k.logical : k.page, s);
     return -1;
   }
-  return ((long long)page * p.hkv + h) * p.page_size + (j - logical * p.page_size);
+  return ((long long)k.page * p.hkv + h) * p.page_size + k.offset;
 }
 
 // Partial states: acc [split][slot][D], then (m, l) [split][slot], slot = (s max_rows + row) Hq + head.
@@ -173,57 +185,89 @@ __device__ __forceinline__ float2 *partial_ml(const WindowAttentionParams &p, lo
   return reinterpret_cast<float2 *>(static_cast<float *>(p.workspace) + splits * slots * p.d) + split * slots + slot;
 }
 
+// Add a state's weighted part: ml its (maximum, sum), m the maximum over all.
+__device__ __forceinline__ void join_part(const float2 &ml, const float4 &x, float m, float &l, float4 &o) {
+  const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
+  l = fmaf(ml.y, f, l);
+  o.x = fmaf(x.x, f, o.x);
+  o.y = fmaf(x.y, f, o.y);
+  o.z = fmaf(x.z, f, o.z);
+  o.w = fmaf(x.w, f, o.w);
+}
+
+// Stores to the same variable in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t in_cta(const void *local, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void store_cluster(const float *local, int rank, const float4 &v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(in_cta(local, rank)), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void store_cluster(const float2 *local, int rank, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(in_cta(local, rank)), "f"(a), "f"(b) : "memory");
+}
+
 // ---- decode: one row per sequence --------------------------------------------------------
 
 template <int D>
 struct DecodeCfg {
   static constexpr int kWarps = 4;
-  static constexpr int kStages = 4;                    // 16-key stages of a warp's ring
+  static constexpr int kStages = 2;                    // 16-key stages of a warp's ring
   static constexpr int kStageBytes = 16 * D * 2;       // one of K or V
   static constexpr int kRing = kWarps * kStages * 2 * kStageBytes;
   static constexpr int kMerge = kWarps * (16 * D + 32) * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+  // and the parts that a cluster's CTAs send: a share each of `heads` rows
+  static constexpr int smem(int heads) { return kSmem + (heads * D + 4 * kMaxCluster) * 4; }
 };
 
 // Grid (splits, Hkv x head tiles, sequences), clusters of `cluster` CTAs along
 // the splits; outer = splits / cluster of them meet in the workspace.
 template <typename E, int D>
-__global__ void __launch_bounds__(128) window_decode_kernel(const WindowAttentionParams p, int head_tiles, int cluster) {
+__global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const WindowAttentionParams p, int head_tiles, int cluster) {
   using C = DecodeCfg<D>;
   constexpr int S = C::kStages;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int bad_keys[C::kWarps][S];        // a stage's keys whose page is missing
-  __shared__ float2 cta_ml[16];                 // this CTA's (m, l) per tile row
-  __shared__ float weights[kMaxCluster * 16];   // of the cluster's CTAs
-  __shared__ float total_l[16];
+  __shared__ float2 recv_ml[kMaxCluster][16];   // (m, l) per tile row, from the cluster's CTAs
+  float *recv = reinterpret_cast<float *>(smem + C::kSmem);  // their parts of this CTA's share of the results
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tq = lane & 3;
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   const int s = blockIdx.z, h = blockIdx.y / head_tiles, tile = blockIdx.y % head_tiles;
   const int split = blockIdx.x, splits = gridDim.x;
   const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
-  if (seq.rows == 0) return;  // the same for every CTA of the cluster
+  if (seq.rows == 0) {  // the same for every CTA of the cluster
+    if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    return;
+  }
   const int g = p.hq / p.hkv, head0 = h * g + tile * 16, heads = min(16, g - tile * 16);
   const Visible vis = visible_keys(p, seq.first, seq.first);
-  // Whole 64-key steps per split, so that the four warps share each evenly.
-  const int chunk = ((vis.count + splits - 1) / splits + 63) / 64 * 64;
+  const int chunk = ((vis.count + splits - 1) / splits + 15) / 16 * 16;
   const int v0 = min(vis.count, split * chunk), v1 = min(vis.count, v0 + chunk);
   const int groups = (v1 - v0 + 15) / 16;
   const int mine = groups > warp ? (groups - warp + C::kWarps - 1) / C::kWarps : 0;
 
   unsigned char *ring = smem + warp * (S * 2 * C::kStageBytes);
   const uint32_t ring_addr = smem_u32(ring);
-  // The pool row of this lane's key (lane & 15) of stage i; -1: none.
-  auto lookup = [&](int i) -> long long {
+  // The place of this lane's key (lane & 15) of stage i, looked up one stage
+  // ahead: nothing waits for the table entry until the stage is issued.
+  auto lookup = [&](int i) {
     const int v = v0 + (warp + C::kWarps * i) * 16 + (lane & 15);
-    return i < mine && v < v1 ? pool_row(p, seq.table, vis.key(v), h, s) : -1;
+    return i < mine && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
   };
   constexpr int kChunks = D / 8;               // 16-byte chunks of a row
   constexpr int kLoads = 16 * kChunks / 32;    // of K (and of V) per lane and stage
-  long long next_row = lookup(0);
+  KeyPlace next = lookup(0);
   auto issue = [&](int i) {
     const int v = v0 + (warp + C::kWarps * i) * 16 + (lane & 15);
-    const unsigned bad = __ballot_sync(0xffffffffu, next_row < 0 && i < mine && v < v1) & 0xffffu;
+    const long long next_row = v < v1 ? pool_row(p, next, h, s) : -1;
+    const unsigned bad = __ballot_sync(0xffffffffu, next_row < 0 && v < v1) & 0xffffu;
+    next = lookup(i + 1);
     if (lane == 0) bad_keys[warp][i % S] = (int)bad;
     const uint32_t dst = ring_addr + (i % S) * 2 * C::kStageBytes;
 #pragma unroll
@@ -236,7 +280,6 @@ __global__ void __launch_bounds__(128) window_decode_kernel(const WindowAttentio
       cp_async16(dst + to, static_cast<const E *>(p.k_pool) + off, bytes);
       cp_async16(dst + C::kStageBytes + to, static_cast<const E *>(p.v_pool) + off, bytes);
     }
-    next_row = lookup(i + 1);
   };
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) {
@@ -355,6 +398,7 @@ __global__ void __launch_bounds__(128) window_decode_kernel(const WindowAttentio
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = gq + 8 * half;
+    if (r >= heads) break;
 #pragma unroll
     for (int dt = 0; dt < D / 8; ++dt)
       *reinterpret_cast<float2 *>(w_acc + (warp * 16 + r) * D + dt * 8 + 2 * tq) =
@@ -362,81 +406,58 @@ __global__ void __launch_bounds__(128) window_decode_kernel(const WindowAttentio
     if (tq == 0) w_ml[warp * 16 + r] = make_float2(m_run[half], l_run[half]);
   }
   __syncthreads();
-  for (int i = tid; i < heads * D; i += 128) {
+  // Join the warps' states, then the CTAs': CTA c of the cluster owns the
+  // elements [c share, (c + 1) share) of the heads x D results; every CTA
+  // stores its part of them, and its (m, l), in the owner's shared memory, and
+  // after one barrier each owner joins what it was sent.
+  const int crank = split % cluster, outer = split / cluster, outers = splits / cluster;
+  const int share = ((heads * D + cluster - 1) / cluster + 3) & ~3;
+  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
+  const long long slot0 = (long long)s * p.max_rows * p.hq + head0;
+  auto finish = [&](int i, const float4 &o, float m, float l) {  // elements i .. i + 3, of one row
+    if (outers > 1) {
+      const int r = i / D;
+      *reinterpret_cast<float4 *>(partial_acc(p, slots, outer, slot0 + r) + i % D) = o;
+      if (i % D == 0) *partial_ml(p, slots, outers, outer, slot0 + r) = make_float2(m, l);
+    } else {
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
+      *reinterpret_cast<uint2 *>(static_cast<E *>(p.out) + seq.start * p.out_stride + (long long)head0 * D + i) =
+          make_uint2(pack2(o.x * inv, o.y * inv, E()), pack2(o.z * inv, o.w * inv, E()));
+    }
+  };
+  if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
+  for (int i = tid * 4; i < heads * D; i += 128 * 4) {
     const int r = i / D;
-    float m = -INFINITY;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < C::kWarps; ++w) m = fmaxf(m, w_ml[w * 16 + r].x);
-    float l = 0.0f, o = 0.0f;
 #pragma unroll
-    for (int w = 0; w < C::kWarps; ++w) {
-      const float2 ml = w_ml[w * 16 + r];
-      const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
-      l = fmaf(ml.y, f, l);
-      o = fmaf(w_acc[w * 16 * D + i], f, o);
+    for (int w = 0; w < C::kWarps; ++w) join_part(w_ml[w * 16 + r], *reinterpret_cast<const float4 *>(w_acc + w * 16 * D + i), m, l, o);
+    if (cluster == 1) {
+      finish(i, o, m, l);
+      continue;
     }
-    w_acc[i] = o;  // only this thread reads element i of warp 0's state
-    if (i % D == 0) cta_ml[r] = make_float2(m, l);
+    const int owner = i / share;
+    store_cluster(recv + crank * share + (i - owner * share), owner, o);
+    if (i % D / 4 < cluster) store_cluster(&recv_ml[crank][r], i % D / 4, m, l);
+    if (D / 4 < cluster && i % D == 0)
+      for (int c = D / 4; c < cluster; ++c) store_cluster(&recv_ml[crank][r], c, m, l);
   }
-  __syncthreads();
-
-  // Join the CTAs of the cluster: each takes a share of the elements and reads
-  // them from every CTA.
-  const int crank = split % cluster, outer = split / cluster, outers = splits / cluster;
-  if (cluster > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-  for (int i = tid; i < cluster * 16; i += 128) {
-    float2 ml;
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(&cta_ml[i % 16])), "r"(i / 16));
-    if (i % 16 < heads)
-      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml.x), "=f"(ml.y) : "r"(a) : "memory");
-    else
-      ml = make_float2(-INFINITY, 0.0f);
-    weights[i] = ml.x;
-    reinterpret_cast<float2 *>(w_ml)[i] = ml;  // cluster * 16 pairs: within the merge area (asserted at launch)
-  }
-  __syncthreads();
-  if (tid < 16) {
-    float m = -INFINITY;
-    for (int c = 0; c < cluster; ++c) m = fmaxf(m, weights[c * 16 + tid]);
-    float l = 0.0f;
-    for (int c = 0; c < cluster; ++c) {
-      const float2 ml = w_ml[c * 16 + tid];
-      const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
-      weights[c * 16 + tid] = f;
-      l = fmaf(ml.y, f, l);
-    }
-    total_l[tid] = l;
-    const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-    if (outers > 1 && crank == 0 && tid < heads)
-      *partial_ml(p, slots, outers, outer, (long long)s * p.max_rows * p.hq + head0 + tid) = make_float2(m, l);
-  }
-  __syncthreads();
-  const int share = (heads * D + cluster - 1) / cluster;
-  const int e1 = min(heads * D, (crank + 1) * share);
-  for (int i = crank * share + tid; i < e1; i += 128) {
+  if (cluster == 1) return;
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int e0 = crank * share, e1 = min(heads * D, e0 + share);
+  for (int i = e0 + tid * 4; i < e1; i += 128 * 4) {
     const int r = i / D;
-    float o = 0.0f;
-    for (int c = 0; c < cluster; ++c) {
-      uint32_t a;
-      float x;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(w_acc + i)), "r"(c));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(a) : "memory");
-      o = fmaf(x, weights[c * 16 + r], o);
-    }
-    if (outers > 1) {
-      const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-      partial_acc(p, slots, outer, (long long)s * p.max_rows * p.hq + head0 + r)[i % D] = o;
-    } else {
-      const float l = total_l[r];
-      store1(p.out, seq.start * p.out_stride + (long long)head0 * D + i, l > 0.0f || l != l ? o / l : 0.0f, E());
-    }
-  }
-  if (cluster > 1) {
-    // No CTA's memory goes away while another reads it.
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < cluster) m = fmaxf(m, recv_ml[c][r].x);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < cluster) join_part(recv_ml[c][r], *reinterpret_cast<const float4 *>(recv + c * share + i - e0), m, l, o);
+    finish(i, o, m, l);
   }
 }
 
@@ -470,7 +491,7 @@ __device__ __noinline__ void slow_row(const WindowAttentionParams &p, const Sequ
   for (int v = v0; v < v1; ++v) {
     const int j = vis.key(v);
     if (j > pos || (pos - j >= p.window && j >= p.sinks)) continue;
-    const long long at = pool_row(p, seq.table, j, h, s);
+    const long long at = pool_row(p, find_key(p, seq.table, j), h, s);
     if (at < 0) continue;
     const E *k = static_cast<const E *>(p.k_pool) + at * D, *x = static_cast<const E *>(p.v_pool) + at * D;
     float dot = 0.0f;
@@ -522,7 +543,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
       const int at = tid + C::kThreads * e, r = at / kChunks, c = at % kChunks;
       if (BN * kChunks % C::kThreads != 0 && r >= BN) break;
       const int v = v0 + i * BN + r;
-      const long long row = v < v1 ? pool_row(p, seq.table, vis.key(v), h, s) : -1;
+      const long long row = v < v1 ? pool_row(p, find_key(p, seq.table, vis.key(v)), h, s) : -1;
       if (c == 0) bad_keys[i % C::kStages][r] = row < 0;
       const long long off = row < 0 ? 0 : row * D + c * 8;
       const int to = tile_offset<D>(r, c);
@@ -718,34 +739,42 @@ __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
 
 // ---- joining splits ----------------------------------------------------------------------
 
-// One warp per (sequence, row, head): out = sum_i w_i acc_i / sum_i w_i l_i,
-// w_i = 2^(m_i - max m).
+// One thread per element, D of them per (sequence, row, head): out =
+// sum_i w_i acc_i / sum_i w_i l_i, w_i = 2^(m_i - max m). All partial sums are
+// read before they are needed; those of empty splits hold nothing and are
+// left out by their weight.
 template <typename E>
 __global__ void __launch_bounds__(128) window_join_kernel(const WindowAttentionParams p, int splits) {
   const int lane = threadIdx.x & 31;
   pdl_wait();
-  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-  const long long slot = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   pdl_launch_dependents();
+  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
+  const int lanes = p.d < 32 ? 32 : p.d;  // threads per slot: whole warps
+  const long long index = (long long)blockIdx.x * 128 + threadIdx.x;
+  const long long slot = index / lanes;
+  const int d = (int)(index % lanes);
   if (slot >= slots) return;
   const int head = (int)(slot % p.hq), row = (int)(slot / p.hq % p.max_rows), s = (int)(slot / p.hq / p.max_rows);
+  float2 ml = lane < splits ? __ldcg(partial_ml(p, slots, splits, lane, slot)) : make_float2(-INFINITY, 0.0f);
+  float x[kMaxOuter];
+  const float *acc = partial_acc(p, slots, 0, slot) + (d < p.d ? d : 0);
+#pragma unroll
+  for (int i = 0; i < kMaxOuter; ++i)
+    if (i < splits) x[i] = __ldcg(acc + i * slots * p.d);
   const Sequence seq = load_sequence(p, s, false);
   if (row >= seq.rows) return;
-  const float2 ml = lane < splits ? __ldcg(partial_ml(p, slots, splits, lane, slot)) : make_float2(-INFINITY, 0.0f);
   const float m = warp_max(ml.x);
   const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
-  // A state without weight is skipped whatever its sum (a NaN sum stays NaN).
+  // A state without weight counts by its sum alone: 0, or NaN.
   const float l = warp_sum(ml.x == -INFINITY ? ml.y : ml.y * w);
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  for (int d0 = 0; d0 < p.d; d0 += 32) {
-    const int d = d0 + lane;
-    float o = 0.0f;
-    for (int i = 0; i < splits; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      if (wi != 0.0f && d < p.d) o = fmaf(__ldcg(partial_acc(p, slots, i, slot) + d), wi, o);
-    }
-    if (d < p.d) store1(p.out, (seq.start + row) * p.out_stride + (long long)head * p.d + d, o * inv, E());
+  float o = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxOuter; ++i) {
+    const float wi = __shfl_sync(0xffffffffu, w, i);
+    if (i < splits && wi != 0.0f) o = fmaf(x[i], wi, o);
   }
+  if (d < p.d) store1(p.out, (seq.start + row) * p.out_stride + (long long)head * p.d + d, o * inv, E());
 }
 
 // ---- launches ----------------------------------------------------------------------------
@@ -761,19 +790,34 @@ size_t partial_bytes(int sequences, int max_rows, int hq, int d, int outer) {
   return outer <= 1 ? 0 : (size_t)outer * sequences * max_rows * hq * (d + 2) * sizeof(float);
 }
 
-// keys: the most keys a row can see. Splits grow while the GPU has room for
-// twice as many CTAs and each still has a few steps of keys.
-Plan make_plan(int sequences, int max_rows, int hq, int hkv, long long keys, int num_sms, int max_cluster) {
+// keys: the most keys a row can see.
+Plan make_plan(int sequences, int max_rows, int hq, int hkv, long long keys, int num_sms) {
   const int g = hq / hkv;
   Plan plan{max_rows == 1, 1, 1, 1};
   plan.tiles = plan.decode ? (g + 15) / 16 : (int)(((long long)max_rows * g + 127) / 128);
   const long long ctas = (long long)sequences * hkv * plan.tiles;
-  const long long room = 2 * num_sms;
-  if (plan.decode)
-    while (plan.cluster < max_cluster && ctas * plan.cluster < room && keys > 64 * plan.cluster) plan.cluster *= 2;
-  const long long steps = plan.decode ? keys / (64 * plan.cluster) : keys / 64;
-  while (plan.outer < kMaxOuter && ctas * plan.cluster * plan.outer * 2 <= room && steps > 4 * plan.outer)
-    plan.outer *= 2;
+  const long long slots = (plan.decode ? kDecodePerSm : 2) * num_sms;  // CTAs that run at the same time
+  if (!plan.decode) {
+    while (plan.outer < kMaxOuter && ctas * plan.outer * 2 <= slots && keys > 256 * plan.outer) plan.outer *= 2;
+    return plan;
+  }
+  // Few CTAs: as many splits as run at once, each with one step of keys for
+  // its four warps at least. Many: a few rounds of CTAs, which evens out
+  // sequences of different lengths, each with eight steps at least.
+  long long splits;
+  if (2 * ctas <= slots) {
+    splits = slots / ctas;
+    if (splits * 64 > keys) splits = (keys + 63) / 64;
+  } else {
+    splits = (5 * slots / 2 + ctas - 1) / ctas;
+    if (splits * 512 > keys) splits = (keys + 511) / 512;
+  }
+  if (splits <= kMaxCluster || keys < 256 * splits) {
+    plan.cluster = (int)(splits < kMaxCluster ? splits : kMaxCluster);
+  } else {
+    plan.cluster = kMaxCluster / 2;
+    plan.outer = (int)(splits / plan.cluster < kMaxOuter ? splits / plan.cluster : kMaxOuter);
+  }
   return plan;
 }
 
@@ -782,70 +826,27 @@ long long visible_bound(long long window, long long sinks, int max_rows, long lo
   return keys < capacity ? keys : capacity;
 }
 
-// The largest cluster of decode CTAs this device runs (16 is not portable), set up once.
-template <typename E, int D>
-cudaError_t decode_cluster_limit(int *limit) {
+// Allows a kernel its dynamic shared memory, once per device.
+cudaError_t allow_smem(const void *kernel, int bytes) {
   static std::mutex mu;
-  static std::unordered_map<int, int> limits;
+  static std::map<std::pair<int, const void *>, bool> done;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   std::lock_guard<std::mutex> lock(mu);
-  auto it = limits.find(dev);
-  if (it == limits.end()) {
-    auto kernel = window_decode_kernel<E, D>;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<D>::kSmem);
-    if (e != cudaSuccess) return e;
-    int n = 8;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
-      cudaLaunchConfig_t probe = {};
-      probe.gridDim = dim3(kMaxCluster, 1, 1);
-      probe.blockDim = dim3(128);
-      probe.dynamicSmemBytes = DecodeCfg<D>::kSmem;
-      cudaLaunchAttribute a;
-      a.id = cudaLaunchAttributeClusterDimension;
-      a.val.clusterDim.x = kMaxCluster;
-      a.val.clusterDim.y = a.val.clusterDim.z = 1;
-      probe.attrs = &a;
-      probe.numAttrs = 1;
-      int clusters = 0;
-      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &probe) == cudaSuccess && clusters > 0) n = kMaxCluster;
-    }
-    (void)cudaGetLastError();
-    it = limits.emplace(dev, n).first;
-  }
-  *limit = it->second;
-  return cudaSuccess;
-}
-
-template <typename E, int D>
-cudaError_t prompt_setup() {
-  static std::mutex mu;
-  static std::unordered_map<int, bool> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(mu);
-  if (done[dev]) return cudaSuccess;
-  e = cudaFuncSetAttribute(window_prompt_kernel<E, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptCfg<D>::kSmem);
-  if (e == cudaSuccess) done[dev] = true;
+  bool &set = done[{dev, kernel}];
+  if (!set && (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) == cudaSuccess)
+    set = true;
   return e;
 }
 
 template <typename E, int D>
 cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t stream, bool pdl) {
-  static_assert(DecodeCfg<D>::kMerge <= DecodeCfg<D>::kSmem, "warp states fit over the rings");
-  static_assert(kMaxCluster * 16 * 8 <= DecodeCfg<D>::kSmem - DecodeCfg<D>::kWarps * 16 * D * 4,
-                "the cluster's (m, l) pairs fit behind the warp states");
-  int limit = 8;
-  cudaError_t e;
-  if (p.max_rows == 1) {
-    if ((e = decode_cluster_limit<E, D>(&limit)) != cudaSuccess) return e;
-  } else if ((e = prompt_setup<E, D>()) != cudaSuccess) {
-    return e;
-  }
+  using C = DecodeCfg<D>;
+  static_assert(C::kMerge <= C::kSmem, "warp states fit over the rings");
+  static_assert(kDecodePerSm * (C::smem(16) + 1024 + 1280) <= 228 * 1024, "CTAs that an SM holds");
   const long long keys = visible_bound(p.window, p.sinks, p.max_rows, p.capacity);
-  Plan plan = make_plan(p.sequences, p.max_rows, p.hq, p.hkv, keys, num_sms, limit);
+  Plan plan = make_plan(p.sequences, p.max_rows, p.hq, p.hkv, keys, num_sms);
   while (plan.outer > 1 &&
          (p.workspace == nullptr ||
           partial_bytes(p.sequences, p.max_rows, p.hq, D, plan.outer) > p.workspace_bytes))
@@ -859,26 +860,32 @@ cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t str
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   };
+  cudaError_t e;
   if (plan.decode) {
+    const auto kernel = window_decode_kernel<E, D>;
+    if ((e = allow_smem(reinterpret_cast<const void *>(kernel), C::smem(16))) != cudaSuccess) return e;
+    const int g = p.hq / p.hkv;
     cfg.gridDim = dim3(plan.cluster * plan.outer, p.hkv * plan.tiles, p.sequences);
     cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = DecodeCfg<D>::kSmem;
+    cfg.dynamicSmemBytes = C::smem(g < 16 ? g : 16);
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = plan.cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
     add_pdl();
-    e = cudaLaunchKernelEx(&cfg, window_decode_kernel<E, D>, p, plan.tiles, plan.cluster);
+    e = cudaLaunchKernelEx(&cfg, kernel, p, plan.tiles, plan.cluster);
   } else {
+    const auto kernel = window_prompt_kernel<E, D>;
+    if ((e = allow_smem(reinterpret_cast<const void *>(kernel), PromptCfg<D>::kSmem)) != cudaSuccess) return e;
     cfg.gridDim = dim3((unsigned)(plan.tiles * plan.outer), p.hkv, p.sequences);
     cfg.blockDim = dim3(PromptCfg<D>::kThreads);
     cfg.dynamicSmemBytes = PromptCfg<D>::kSmem;
     add_pdl();
-    e = cudaLaunchKernelEx(&cfg, window_prompt_kernel<E, D>, p, plan.outer);
+    e = cudaLaunchKernelEx(&cfg, kernel, p, plan.outer);
   }
   if (e != cudaSuccess || plan.outer == 1) return e;
   const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-  cfg.gridDim = dim3((unsigned)((slots + 3) / 4));
+  cfg.gridDim = dim3((unsigned)((slots * (D < 32 ? 32 : D) + 127) / 128));
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 0;
@@ -903,14 +910,9 @@ size_t window_attention_workspace_bytes(int sequences, int max_rows, int hq, int
                                         long long sinks, int num_sms) {
   if (sequences <= 0 || max_rows <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || d <= 0 || window <= 0 || sinks < 0)
     return 0;
-  const long long keys = visible_bound(window, sinks, max_rows, 0x7fffffffll);
-  size_t most = 0;
-  for (int cluster = 8; cluster <= kMaxCluster; cluster *= 2) {
-    const Plan plan = make_plan(sequences, max_rows, hq, hkv, keys, num_sms, cluster);
-    const size_t bytes = partial_bytes(sequences, max_rows, hq, d, plan.outer);
-    most = bytes > most ? bytes : most;
-  }
-  return most;
+  const Plan plan =
+      make_plan(sequences, max_rows, hq, hkv, visible_bound(window, sinks, max_rows, 0x7fffffffll), num_sms);
+  return partial_bytes(sequences, max_rows, hq, d, plan.outer);
 }
 
 cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, int num_sms, cudaStream_t stream,
@@ -923,7 +925,11 @@ cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, i
   if ((long long)p.hkv * ((g + 15) / 16) > 65535 || (long long)p.max_rows * g > (1ll << 30) / kMaxOuter ||
       (long long)p.sequences * p.max_rows > (1ll << 32) / p.hq)
     return cudaErrorInvalidValue;
-  return bf16 ? dispatch<__nv_bfloat16>(p, num_sms, stream, pdl) : dispatch<__half>(p, num_sms, stream, pdl);
+  WindowAttentionParams q = p;
+  q.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (p.page_size == 1 << i) q.page_shift = i;
+  return bf16 ? dispatch<__nv_bfloat16>(q, num_sms, stream, pdl) : dispatch<__half>(q, num_sms, stream, pdl);
 }
 
 }  // namespace tmc

@@ -31,6 +31,7 @@ struct WindowAttentionParams {
   void *workspace;  // partial results of splits that meet in a second kernel
   size_t workspace_bytes;
   TmcDeviceStatus *status;
+  int page_shift;  // set by the launch: log2(page_size), or -1
 };
 
 // Bytes with which a launch runs as many splits as it can use (0: it needs none).
