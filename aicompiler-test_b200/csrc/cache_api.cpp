@@ -3,6 +3,7 @@
 // include/tmc_cuda.h).
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 #include <string>
 
 #include "api_util.hpp"
@@ -42,6 +43,34 @@ class OnDeviceOf {
 };
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Arguments in 8-byte slots, in declaration order.
+class Slots {
+ public:
+  explicit Slots(const int64_t *slots) : at_(slots) {}
+  template <typename T>
+  T *pointer() {
+    return reinterpret_cast<T *>(static_cast<uintptr_t>(*at_++));
+  }
+  int64_t wide() { return *at_++; }
+  int whole() {
+    const int64_t v = *at_++;
+    if (v < INT32_MIN || v > INT32_MAX) fits_ = false;
+    return static_cast<int>(v);
+  }
+  float real() {
+    const uint32_t bits = static_cast<uint32_t>(*at_++);
+    float v;
+    std::memcpy(&v, &bits, sizeof v);
+    return v;
+  }
+  bool fits() const { return fits_; }  // every whole number was a 32-bit one
+
+ private:
+  const int64_t *at_;
+  bool fits_ = true;
+};
+const char *const kWide = "an integer argument does not fit 32 bits";
 
 }  // namespace
 
@@ -209,6 +238,96 @@ int tmc_k_kv_compact(void *const *pools, int layers, int dtype, int pool_pages, 
   const cudaError_t e = tmc::launch_kv_compact(p, dtype == TMC_BF16, static_cast<cudaStream_t>(stream));
   if (e == cudaErrorInvalidValue) return fail(TMC_ERR_UNSUPPORTED, "compact: unsupported shape");
   return e == cudaSuccess ? ok() : cuda_fail(e, "compact launch");
+}
+
+int tmc_k_window_attention_slots(const int64_t *slots) {
+  if (!slots) return fail(TMC_ERR_INVALID, "null pointer");
+  Slots a(slots);
+  const auto *q = a.pointer<const void>();
+  const int64_t q_stride = a.wide();
+  auto *out = a.pointer<void>();
+  const int64_t out_stride = a.wide();
+  const auto *k = a.pointer<const void>();
+  const auto *v = a.pointer<const void>();
+  const int dtype = a.whole();
+  const auto *table = a.pointer<const int32_t>();
+  const int table_stride = a.whole();
+  const auto *table_rows = a.pointer<const int32_t>();
+  const auto *row_starts = a.pointer<const int32_t>();
+  const auto *first = a.pointer<const int32_t>();
+  int n[11];  // sequences .. sinks
+  for (int &x : n) x = a.whole();
+  const float scale = a.real();
+  auto *workspace = a.pointer<void>();
+  const int64_t bytes = a.wide();
+  auto *status = a.pointer<void>();
+  auto *stream = a.pointer<void>();
+  if (!a.fits() || bytes < 0) return fail(TMC_ERR_INVALID, kWide);
+  return tmc_k_window_attention(q, q_stride, out, out_stride, k, v, dtype, table, table_stride, table_rows, row_starts,
+                                first, n[0], n[1], n[2], n[3], n[4], n[5], n[6], n[7], n[8], n[9], n[10], scale,
+                                workspace, static_cast<size_t>(bytes), status, stream);
+}
+
+int tmc_k_token_logprobs_slots(const int64_t *slots) {
+  if (!slots) return fail(TMC_ERR_INVALID, "null pointer");
+  Slots a(slots);
+  const auto *logits = a.pointer<const void>();
+  const int dtype = a.whole();
+  const int64_t stride = a.wide();
+  const auto *targets = a.pointer<const int32_t>();
+  const int rows = a.whole();
+  const int vocab = a.whole();
+  auto *logprobs = a.pointer<float>();
+  auto *entropy = a.pointer<float>();
+  auto *ranks = a.pointer<int32_t>();
+  const int top = a.whole();
+  auto *ids = a.pointer<int32_t>();
+  auto *values = a.pointer<float>();
+  auto *status = a.pointer<void>();
+  auto *stream = a.pointer<void>();
+  if (!a.fits()) return fail(TMC_ERR_INVALID, kWide);
+  return tmc_k_token_logprobs(logits, dtype, stride, targets, rows, vocab, logprobs, entropy, ranks, top, ids, values,
+                              status, stream);
+}
+
+int tmc_k_kv_copy_pages_slots(const int64_t *slots) {
+  if (!slots) return fail(TMC_ERR_INVALID, "null pointer");
+  Slots a(slots);
+  auto *pools = a.pointer<void *const>();
+  const int pool_count = a.whole();
+  const int pool_pages = a.whole();
+  const int64_t page_bytes = a.wide();
+  const auto *src = a.pointer<const int32_t>();
+  const auto *dst = a.pointer<const int32_t>();
+  const int count = a.whole();
+  auto *status = a.pointer<void>();
+  auto *stream = a.pointer<void>();
+  if (!a.fits() || page_bytes < 0) return fail(TMC_ERR_INVALID, kWide);
+  return tmc_k_kv_copy_pages(pools, pool_count, pool_pages, static_cast<size_t>(page_bytes), src, dst, count, status,
+                             stream);
+}
+
+int tmc_k_kv_compact_slots(const int64_t *slots) {
+  if (!slots) return fail(TMC_ERR_INVALID, "null pointer");
+  Slots a(slots);
+  auto *pools = a.pointer<void *const>();
+  int n[6];  // layers .. page_size
+  for (int &x : n) x = a.whole();
+  const auto *src = a.pointer<const int32_t>();
+  const int src_count = a.whole();
+  const auto *dst = a.pointer<const int32_t>();
+  const int dst_count = a.whole();
+  const auto *keep = a.pointer<const int32_t>();
+  const int count = a.whole();
+  const int first = a.whole();
+  const auto *cos = a.pointer<const float>();
+  const auto *sin = a.pointer<const float>();
+  const int rope_rows = a.whole();
+  auto *status = a.pointer<void>();
+  auto *stream = a.pointer<void>();
+  if (!a.fits()) return fail(TMC_ERR_INVALID, kWide);
+  return tmc_k_kv_compact(pools, n[0], n[1], n[2], n[3], n[4], n[5], src, src_count, dst, dst_count, keep, count, first,
+                          cos, sin, rope_rows, status, stream);
 }
 
 }  // extern "C"

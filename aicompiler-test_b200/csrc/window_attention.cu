@@ -812,9 +812,13 @@ Plan make_plan(int sequences, int max_rows, int hq, int hkv, long long keys, int
     splits = (5 * slots / 2 + ctas - 1) / ctas;
     if (splits * 512 > keys) splits = (keys + 511) / 512;
   }
-  if (splits <= kMaxCluster || keys < 256 * splits) {
+  // Beyond a cluster the splits' states meet in the workspace, at the cost of
+  // a second launch: that takes four clusters' worth of them, of 256 keys each.
+  const long long wide = splits < keys / 256 ? splits : keys / 256;
+  if (wide < 4 * kMaxCluster) {
     plan.cluster = (int)(splits < kMaxCluster ? splits : kMaxCluster);
   } else {
+    splits = wide;
     plan.cluster = kMaxCluster / 2;
     plan.outer = (int)(splits / plan.cluster < kMaxOuter ? splits / plan.cluster : kMaxOuter);
   }

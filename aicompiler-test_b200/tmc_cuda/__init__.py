@@ -13,7 +13,9 @@ host floats.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+import struct
 from ctypes import (POINTER, c_char_p, c_float, c_int, c_int32, c_size_t, c_uint32, c_uint64,
                     c_void_p)
 
@@ -114,6 +116,8 @@ _sig("tmc_k_token_logprobs", c_int, c_void_p, c_int, ctypes.c_int64, c_void_p, c
 _sig("tmc_k_kv_copy_pages", c_int, c_void_p, c_int, c_int, c_size_t, c_void_p, c_void_p, c_int, c_void_p, c_void_p)
 _sig("tmc_k_kv_compact", c_int, c_void_p, *[c_int] * 6, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int,
      c_void_p, c_void_p, c_int, c_void_p, c_void_p)
+for _name in ("window_attention", "token_logprobs", "kv_copy_pages", "kv_compact"):
+    _sig(f"tmc_k_{_name}_slots", c_int, c_char_p)
 
 
 def last_error() -> str:
@@ -149,11 +153,14 @@ class Runtime:
         check(lib.tmc_runtime_create(device, ctypes.byref(h)))
         self.handle = h
         self.device = device
+        self._stream = lib.tmc_runtime_stream(h)  # both stay the runtime's until it is closed
+        self._status_ptr = lib.tmc_runtime_status_ptr(h)
 
     def close(self):
         if self.handle:
             lib.tmc_runtime_destroy(self.handle)
             self.handle = c_void_p()
+            self._stream = self._status_ptr = None
 
     def __del__(self):
         try:
@@ -163,11 +170,11 @@ class Runtime:
 
     @property
     def stream(self):
-        return lib.tmc_runtime_stream(self.handle)
+        return self._stream
 
     @property
     def status_ptr(self):
-        return lib.tmc_runtime_status_ptr(self.handle)
+        return self._status_ptr
 
     def synchronize(self):
         check(lib.tmc_runtime_synchronize(self.handle))
@@ -213,6 +220,13 @@ class Buffer:
     @property
     def ptr(self) -> int:
         return lib.tmc_buffer_device_ptr(self.handle)
+
+    def data_ptr(self) -> int:
+        return lib.tmc_buffer_device_ptr(self.handle)
+
+    @property
+    def nbytes(self) -> int:
+        return self.count * (4 if self.dtype in (F32, I32) else 2)
 
     def read(self) -> np.ndarray:
         """Logical float values."""
@@ -409,29 +423,31 @@ def paged_attention_f16(rt: Runtime, q: Buffer, out: Buffer, k_pool: Buffer, v_p
         rt.stream))
 
 
-# Serving-cache kernels: arrays are Buffers or objects with data_ptr() and dtype
-# (tensors of another library); `stream` is a cudaStream_t value, the runtime's
-# stream when None.
+# Serving-cache kernels: arrays are Buffers or objects with data_ptr(), dtype and nbytes
+# (tensors of another library); `stream` is a cudaStream_t value, the runtime's stream
+# when None. Their arguments go over as one packed block: converting two dozen of them
+# one by one costs more than the launch.
 
-_DTYPE_NAMES = {"float16": F16, "float32": F32, "bfloat16": BF16}
-
-
-def _ptr(array):
-    if array is None:
-        return None
-    return array.ptr if isinstance(array, Buffer) else array.data_ptr()
-
-
-def _dtype_of(array) -> int:
-    return array.dtype if isinstance(array, Buffer) else _DTYPE_NAMES[str(array.dtype).rpartition(".")[2]]
+_ELEMENT_TYPES = {F16: F16, F32: F32, BF16: BF16, I32: I32}
+_FOREIGN_TYPES = {"float16": F16, "float32": F32, "bfloat16": BF16, "int32": I32}
+_window_attention_slots = struct.Struct("=23qf4x4q").pack
+_token_logprobs_slots = struct.Struct("=14q").pack
+_kv_copy_pages_slots = struct.Struct("=9q").pack
+_kv_compact_slots = struct.Struct("=19q").pack
 
 
-def _nbytes(array) -> int:
-    if isinstance(array, Buffer):
-        return array.count * (4 if array.dtype in (F32, I32) else 2)
-    return array.numel() * array.element_size()
+def _element_type(dtype) -> int:
+    code = _ELEMENT_TYPES.get(dtype)
+    if code is None:
+        code = _ELEMENT_TYPES[dtype] = _FOREIGN_TYPES[str(dtype).rpartition(".")[2]]
+    return code
 
 
+def _address(array) -> int:
+    return 0 if array is None else array.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
 def window_attention_workspace_bytes(sequences: int, max_rows: int, hq: int, hkv: int, d: int, window: int,
                                      sinks: int = 0) -> int:
     return int(lib.tmc_k_window_attention_workspace_bytes(sequences, max_rows, hq, hkv, d, window, sinks))
@@ -443,30 +459,38 @@ def window_attention(rt: Runtime, q, out, k_pool, v_pool, block_table, table_str
                      q_stride: int | None = None, out_stride: int | None = None, workspace=None, stream=None):
     """Attention over the paged cache with a sliding window and `sinks` first positions that
     stay visible, for ragged query rows (tmc_k_window_attention); fp16 or bf16, as q."""
-    check(lib.tmc_k_window_attention(
-        _ptr(q), hq * d if q_stride is None else q_stride, _ptr(out), hq * d if out_stride is None else out_stride,
-        _ptr(k_pool), _ptr(v_pool), _dtype_of(q), _ptr(block_table), table_stride, _ptr(table_rows), _ptr(row_starts),
-        _ptr(first_positions), sequences, rows, max_rows, hq, hkv, d, page_size, pool_pages, capacity, window, sinks,
-        scale, _ptr(workspace), 0 if workspace is None else _nbytes(workspace), rt.status_ptr,
-        rt.stream if stream is None else stream))
+    code = lib.tmc_k_window_attention_slots(_window_attention_slots(
+        q.data_ptr(), hq * d if q_stride is None else q_stride, out.data_ptr(),
+        hq * d if out_stride is None else out_stride, k_pool.data_ptr(), v_pool.data_ptr(), _element_type(q.dtype),
+        block_table.data_ptr(), table_stride, table_rows.data_ptr(), row_starts.data_ptr(), first_positions.data_ptr(),
+        sequences, rows, max_rows, hq, hkv, d, page_size, pool_pages, capacity, window, sinks, scale,
+        _address(workspace), 0 if workspace is None else workspace.nbytes, rt.status_ptr or 0,
+        (rt.stream if stream is None else stream) or 0))
+    if code:
+        check(code)
 
 
 def token_logprobs(rt: Runtime, logits, targets, rows: int, vocab: int, logprobs, entropy=None, ranks=None,
                    top: int = 0, top_ids=None, top_logprobs=None, row_stride: int | None = None, stream=None):
     """Log probability, rank and entropy of one given token per row of logits, with the `top`
     largest alternatives (tmc_k_token_logprobs)."""
-    check(lib.tmc_k_token_logprobs(
-        _ptr(logits), _dtype_of(logits), vocab if row_stride is None else row_stride, _ptr(targets), rows, vocab,
-        _ptr(logprobs), _ptr(entropy), _ptr(ranks), top, _ptr(top_ids) if top else None,
-        _ptr(top_logprobs) if top else None, rt.status_ptr, rt.stream if stream is None else stream))
+    code = lib.tmc_k_token_logprobs_slots(_token_logprobs_slots(
+        logits.data_ptr(), _element_type(logits.dtype), vocab if row_stride is None else row_stride, _address(targets),
+        rows, vocab, _address(logprobs), _address(entropy), _address(ranks), top, _address(top_ids) if top else 0,
+        _address(top_logprobs) if top else 0, rt.status_ptr or 0, (rt.stream if stream is None else stream) or 0))
+    if code:
+        check(code)
 
 
 def kv_copy_pages(rt: Runtime, pools, pool_count: int, pool_pages: int, page_bytes: int, src, dst, count: int,
                   stream=None):
     """Copy page src[i] to page dst[i] of every pool; pools: device array of addresses
     (tmc_k_kv_copy_pages)."""
-    check(lib.tmc_k_kv_copy_pages(_ptr(pools), pool_count, pool_pages, page_bytes, _ptr(src), _ptr(dst), count,
-                                  rt.status_ptr, rt.stream if stream is None else stream))
+    code = lib.tmc_k_kv_copy_pages_slots(_kv_copy_pages_slots(
+        pools.data_ptr(), pool_count, pool_pages, page_bytes, src.data_ptr(), dst.data_ptr(), count,
+        rt.status_ptr or 0, (rt.stream if stream is None else stream) or 0))
+    if code:
+        check(code)
 
 
 def kv_compact(rt: Runtime, pools, layers: int, pool_pages: int, hkv: int, d: int, page_size: int, src_pages,
@@ -474,9 +498,12 @@ def kv_compact(rt: Runtime, pools, layers: int, pool_pages: int, hkv: int, d: in
                rope_sin=None, rope_rows: int = 0, dtype: int = F16, stream=None):
     """Move the kept rows of a sequence together into other pages, keys turned by the distance
     moved (tmc_k_kv_compact)."""
-    check(lib.tmc_k_kv_compact(_ptr(pools), layers, dtype, pool_pages, hkv, d, page_size, _ptr(src_pages), src_count,
-                               _ptr(dst_pages), dst_count, _ptr(keep), count, first, _ptr(rope_cos), _ptr(rope_sin),
-                               rope_rows, rt.status_ptr, rt.stream if stream is None else stream))
+    code = lib.tmc_k_kv_compact_slots(_kv_compact_slots(
+        pools.data_ptr(), layers, dtype, pool_pages, hkv, d, page_size, src_pages.data_ptr(), src_count,
+        dst_pages.data_ptr(), dst_count, keep.data_ptr(), count, first, _address(rope_cos), _address(rope_sin),
+        rope_rows, rt.status_ptr or 0, (rt.stream if stream is None else stream) or 0))
+    if code:
+        check(code)
 
 
 def fill_normal_f16(rt: Runtime, buf: Buffer, seed: int, mean: float, std: float):

@@ -351,6 +351,14 @@ int tmc_k_kv_compact(void *const *pools, int layers, int dtype, int pool_pages, 
                      const int32_t *keep, int count, int first, const float *rope_cos, const float *rope_sin,
                      int rope_rows, void *status, void *stream);
 
+/* The same calls with their arguments in one block of 8-byte slots, in
+ * declaration order: pointers and integers as int64, `scale` as its float bits.
+ * For bindings that pay for every converted argument (the Python package). */
+int tmc_k_window_attention_slots(const int64_t *slots);
+int tmc_k_token_logprobs_slots(const int64_t *slots);
+int tmc_k_kv_copy_pages_slots(const int64_t *slots);
+int tmc_k_kv_compact_slots(const int64_t *slots);
+
 /* Deterministic N(0, std^2) fp16 fill from a counter-based hash generator
  * (synthetic random-init weights without a host round trip). */
 int tmc_k_fill_normal_f16(void *dst, size_t count, uint64_t seed, float mean, float stddev,

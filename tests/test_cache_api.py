@@ -98,3 +98,36 @@ def test_window_attention_workspace_grows_only_where_splits_meet():
     assert need(1, 1, 4, 1, 128, 64, 4) == 0  # nothing to split
     assert need(1, 1, 4, 1, 128, 65536, 4) > 0
     assert need(0, 1, 4, 1, 128, 65536, 4) == 0 == need(1, 1, 4, 3, 128, 65536, 4)
+
+
+def test_integers_beyond_32_bits_are_refused():
+    class Array:
+        def __init__(self, dtype=tmc_cuda.F16):
+            self.dtype, self.nbytes = dtype, 64
+
+        def data_ptr(self):
+            return P
+
+    class Runtime:
+        stream = status_ptr = None
+
+    a, rt = Array(), Runtime()
+    with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
+        tmc_cuda.window_attention(rt, a, a, a, a, a, 4, a, a, a, 1, 1, 1, 4, 2, 128, 16, 8, 64, 1 << 32, 0)
+    with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
+        tmc_cuda.kv_copy_pages(rt, a, 2, 8, 64, a, a, (1 << 32) + 1)
+    with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
+        tmc_cuda.token_logprobs(rt, a, a, 1 << 33, 100, a)
+    with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
+        tmc_cuda.kv_compact(rt, a, 1, 8, 2, 64, 16, a, 4, a, 4, a, 1 << 32)
+    # the same refusals as the C entries give, through the packed form
+    with pytest.raises(tmc_cuda.TmcError, match="window >= 1"):
+        tmc_cuda.window_attention(rt, a, a, a, a, a, 4, a, a, a, 1, 1, 1, 4, 2, 128, 16, 8, 64, 0, 0)
+    with pytest.raises(tmc_cuda.TmcError, match="scale"):
+        tmc_cuda.window_attention(rt, a, a, a, a, a, 4, a, a, a, 1, 1, 1, 4, 2, 128, 16, 8, 64, 9, 0, scale=-0.5)
+    with pytest.raises(tmc_cuda.TmcError, match="top"):
+        tmc_cuda.token_logprobs(rt, a, a, 1, 100, a, top=33, top_ids=a, top_logprobs=a)
+    with pytest.raises(tmc_cuda.TmcError, match="multiple of 8"):
+        tmc_cuda.kv_compact(rt, a, 1, 8, 2, 12, 16, a, 4, a, 4, a, 1)
+    for name in ("window_attention", "token_logprobs", "kv_copy_pages", "kv_compact"):
+        assert getattr(tmc_cuda.lib, f"tmc_k_{name}_slots")(None) == tmc_cuda.ERR_INVALID
