@@ -9,10 +9,14 @@
 // u is summed about the maximum so that a peaked row's small entropy does not
 // come out as a difference of two large numbers.
 //
-// The top alternatives come from the same read: every thread keeps its largest
-// logit as an ordered (value, index) key; the top-th largest of these keys is a
-// lower bound for the row's top-th logit, so only the at most `top` threads
-// whose own largest reaches it are read again, each by a whole warp (from L2).
+// The top alternatives come from the same read. Every thread keeps its largest
+// logit; the top-th largest of each warp's four best of these is reached by at
+// least `top` logits, so it bounds the CTA's top-th logit from below. The few
+// threads whose own largest reaches it are read again (from L2), what reaches
+// the bound is collected, and each of these candidates finds its place by
+// counting the larger ones. Rows with too many candidates (long runs of equal
+// logits) or too few threads with a logit above -inf are read again as a whole,
+// every warp keeping a sorted list.
 //
 // A row is shared by a thread-block cluster when there are few rows; its CTAs
 // hand their (m, s, u), counts and top lists to the cluster's first CTA
@@ -29,6 +33,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+static_assert(kMaxCluster <= kWarps, "a warp for each CTA's list");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -99,11 +104,22 @@ __device__ __forceinline__ Stats warp_join(Stats a) {
   return a;
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 0 below the normal range
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // N logits (index of the first: at) into the running statistics, the count
-// before the target and the thread's largest key.
+// before the target and the thread's largest logit.
 template <int N, bool TOP>
 __device__ __forceinline__ void take(const float (&x)[N], int at, float xt, int target, Stats &st, int &before,
-                                     float &best, int &best_at) {
+                                     int &best_at) {
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
@@ -114,39 +130,34 @@ __device__ __forceinline__ void take(const float (&x)[N], int at, float xt, int 
       st.s *= f;
     }
     st.m = mx;
-    if (TOP) {
-      best = mx;
-      best_at = at;
-    }
+    if (TOP) best_at = at;
   }
   const float m = st.m == -INFINITY ? 0.0f : st.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float d = x[i] - m;
-    const float e = exp2f(d * kLog2e);
+    // A masked logit (-inf) or one far below the maximum: 0 times a finite number.
+    const float d = max_or_nan(x[i] - m, -1e4f);
+    const float e = exp2_fast(d * kLog2e);
     st.s += e;
-    st.u = fmaf(e, fmaxf(d, -1e30f), st.u);  // a masked logit: 0 times a finite number
-    before += (x[i] > xt || (x[i] == xt && at + i < target)) ? 1 : 0;
+    st.u = fmaf(e, d, st.u);
+  }
+  if (at + N <= target) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) before += x[i] >= xt ? 1 : 0;
+  } else if (at > target) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) before += x[i] > xt ? 1 : 0;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) before += (x[i] > xt || (x[i] == xt && at + i < target)) ? 1 : 0;
   }
 }
 
 // Larger logits first, then lower indices; NaN counts as -inf, -0 as 0.
 __device__ __forceinline__ Key order_key(float x, int index) { return argmax_key(__fadd_rn(x, 0.0f), index); }
+__device__ __forceinline__ uint32_t order_value(float x) { return (uint32_t)(order_key(x, 0) >> 32); }
 
 __device__ __forceinline__ Key shfl_key(Key k, int lane) { return __shfl_sync(0xffffffffu, k, lane); }
-// Descending bitonic sort of one key per lane.
-__device__ __forceinline__ Key warp_sort(Key k, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1) {
-#pragma unroll
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      const Key o = __shfl_xor_sync(0xffffffffu, k, step);
-      const bool first = (lane & step) == 0, descending = (lane & size) == 0;
-      k = (first == descending) ? (k > o ? k : o) : (k < o ? k : o);
-    }
-  }
-  return k;
-}
 // The 32 largest of two descending lists of 32 (one key of each per lane), descending.
 __device__ __forceinline__ Key warp_merge(Key a, Key b, int lane) {
   const Key r = shfl_key(b, 31 - lane);
@@ -199,18 +210,33 @@ __device__ __forceinline__ void store_cluster(uint32_t at, Key v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
 
+// How many keys of a descending list of 32 (padded with 0) are larger than k.
+__device__ __forceinline__ int larger_in(const Key *list, Key k) {
+  int n = 0;
+#pragma unroll
+  for (int step = 16; step > 0; step >>= 1)
+    if (list[n + step - 1] > k) n += step;
+  return n + (list[n] > k ? 1 : 0);
+}
+
+constexpr int kWarpBest = 4;           // largest logits per warp that make the bound
+constexpr int kMaxCandidates = kThreads;
+
 // Grid (rows x cluster); the CTAs of a cluster share one row.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobsParams p) {
   using L = Logit<T>;
   constexpr int N = L::kVec;
+  static_assert(kWarps * kWarpBest == 32, "a warp ranks the CTA's best, one per lane");
   __shared__ Stats warp_stats[kWarps];
   __shared__ int warp_before[kWarps];
-  __shared__ Key lists[kWarps * 32];
-  __shared__ Key threshold;
-  __shared__ int flagged[kLogprobsMaxTop];
-  __shared__ int flagged_count;
+  __shared__ uint32_t warp_best[32];
+  __shared__ int flagged[kThreads];
+  __shared__ int flagged_count, candidate_count;
+  __shared__ __align__(16) Key keys[kMaxCandidates];  // candidates, or the warps' lists
+  __shared__ Key sorted[32];                          // the CTA's largest
   __shared__ Part parts[kMaxCluster];
+  __shared__ Stats row_stats;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int csize = (int)cluster_size(), crank = (int)cluster_rank(), row = blockIdx.x / csize;
@@ -223,7 +249,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
   const bool given = target >= 0 && !bad_target;
   const float xt = given ? L::get(x + target) : INFINITY;
 
-  // This CTA's logits [begin, end): whole vectors but for the row's ends. The
+  // This CTA's logits: whole vectors [v0, v1) but for the row's ends. The
   // first `head` logits of the row come before its first 16-byte boundary.
   const int misaligned = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const int head = min(misaligned ? N - misaligned : 0, p.vocab);
@@ -231,16 +257,18 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
   const int per = (vectors + csize - 1) / csize;
   const int v0 = min(vectors, crank * per), v1 = min(vectors, v0 + per);
   const uint4 *body = reinterpret_cast<const uint4 *>(x + head);
+  // The element at either end that this thread takes besides its vectors (-1: none).
+  const int at_head = crank == 0 && tid < head ? tid : -1;
+  const int at_tail = crank == csize - 1 && tid < tail ? head + vectors * N + tid : -1;
 
   Stats st = empty_stats();
   int before = 0;
-  float best = -INFINITY;
   int best_at = -1;  // first index of the vector that holds the thread's largest logit
-  if (crank == 0 && tid < head) {
-    const float one[1] = {L::get(x + tid)};
-    take<1, TOP>(one, tid, xt, target, st, before, best, best_at);
+  if (at_head >= 0) {
+    const float one[1] = {L::get(x + at_head)};
+    take<1, TOP>(one, at_head, xt, target, st, before, best_at);
   }
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 32 / N;
   for (int v = v0 + tid; v < v1; v += kThreads * kUnroll) {
     uint4 raw[kUnroll];
 #pragma unroll
@@ -251,16 +279,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
       if (v + i * kThreads < v1) {
         float f[N];
         L::unpack(raw[i], f);
-        take<N, TOP>(f, head + (v + i * kThreads) * N, xt, target, st, before, best, best_at);
+        take<N, TOP>(f, head + (v + i * kThreads) * N, xt, target, st, before, best_at);
       }
   }
-  if (crank == csize - 1 && tid < tail) {
-    const int at = head + vectors * N + tid;
-    const float one[1] = {L::get(x + at)};
-    take<1, TOP>(one, at, xt, target, st, before, best, best_at);
+  if (at_tail >= 0) {
+    const float one[1] = {L::get(x + at_tail)};
+    take<1, TOP>(one, at_tail, xt, target, st, before, best_at);
   }
 
-  // The CTA's statistics.
+  const uint32_t mine = TOP && best_at >= 0 ? order_value(st.m) : 0u;  // 0: nothing above -inf
   {
     const Stats w = warp_join(st);
 #pragma unroll
@@ -270,147 +297,154 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
       warp_before[warp] = before;
     }
   }
-
-  Key top_key = 0;  // warp 0, lane i: the CTA's i-th largest (0: none)
   if (TOP) {
-    // Keys order by value, then by the lower index. A thread's own largest
-    // element is looked for again in the vector that held it.
-    Key mine = 0;
-    if (best_at >= 0) {
-      mine = order_key(best, best_at);
-      if (best_at >= head && best_at < head + vectors * N) {
-        for (int i = 0; i < N; ++i)
-          if (L::get(x + best_at + i) == best) {
-            mine = order_key(best, best_at + i);
-            break;
-          }
-      }
+    uint32_t left = mine;
+#pragma unroll
+    for (int i = 0; i < kWarpBest; ++i) {
+      const uint32_t best = __reduce_max_sync(0xffffffffu, left);
+      const unsigned holders = __ballot_sync(0xffffffffu, left == best);
+      if (lane == __ffs(holders) - 1) left = 0;
+      if (lane == 0) warp_best[warp * kWarpBest + i] = best;
     }
-    // The top-th largest of the threads' largest keys bounds the CTA's top-th
-    // key from below. Threads that saw only -inf or NaN have no key: their
-    // elements count when there are too few others.
-    lists[warp * 32 + lane] = warp_sort(mine, lane);
-    if (tid == 0) flagged_count = 0;
-    __syncthreads();
-    if (warp == 0) {
-      const Key k = merge_lists(lists, kWarps, lane);
-      if (lane == p.top - 1) threshold = k;
-    }
-    __syncthreads();
-    const Key bound = threshold;
-    Key list = 0;  // this warp's descending list, one key per lane
-    auto offer = [&](Key k) {
-      // Lanes whose key reaches the bound and the full list insert them one
-      // after another.
-      const Key last = shfl_key(list, 31);
-      unsigned want = __ballot_sync(0xffffffffu, k >= bound && k > last);
-      while (want) {
-        const Key c = shfl_key(k, __ffs(want) - 1);
-        want &= want - 1;
-        const int at = __popc(__ballot_sync(0xffffffffu, list > c));
-        const Key up = __shfl_up_sync(0xffffffffu, list, 1);
-        list = lane < at ? list : (lane == at ? c : up);
-      }
-    };
-    if (bound != 0) {
-      if (mine >= bound) flagged[atomicAdd(&flagged_count, 1)] = tid;
-      __syncthreads();
-      const int n = flagged_count;
-      for (int f = warp; f < n; f += kWarps) {
-        const int t = flagged[f];
-        // thread t's elements, spread over the lanes
-        const int mine_vectors = v1 - v0 > t ? (v1 - v0 - t + kThreads - 1) / kThreads : 0;
-        for (int e0 = 0; e0 < mine_vectors * N; e0 += 32) {
-          const int e = e0 + lane;
-          Key k = 0;
-          if (e < mine_vectors * N) {
-            const int at = head + (v0 + t + e / N * kThreads) * N + e % N;
-            k = order_key(L::get(x + at), at);
-          }
-          offer(k);
-        }
-        Key k = 0;
-        if (lane == 0 && crank == 0 && t < head) k = order_key(L::get(x + t), t);
-        if (lane == 1 && crank == csize - 1 && t < tail) {
-          const int at = head + vectors * N + t;
-          k = order_key(L::get(x + at), at);
-        }
-        offer(k);
-      }
-    } else {
-      // Fewer than `top` threads saw a logit above -inf (a short or masked
-      // row): every element is offered.
-      __syncthreads();
-      const int e1 = (v1 - v0) * N;
-      for (int e0 = warp * 32; e0 < e1; e0 += kThreads) {
-        const int at = head + v0 * N + e0 + lane;
-        offer(e0 + lane < e1 ? order_key(L::get(x + at), at) : 0ull);
-      }
-      Key k = 0;
-      if (warp == 0 && crank == 0 && lane < head) k = order_key(L::get(x + lane), lane);
-      offer(k);
-      k = 0;
-      if (warp == 0 && crank == csize - 1 && lane < tail) {
-        const int at = head + vectors * N + lane;
-        k = order_key(L::get(x + at), at);
-      }
-      offer(k);
-    }
-    lists[warp * 32 + lane] = list;
+    if (tid == 0) flagged_count = candidate_count = 0;
+    if (tid < 32) sorted[tid] = 0;
   }
   __syncthreads();
-  if (warp == 0) {
-    if (TOP) top_key = merge_lists(lists, kWarps, lane);
+  if (TOP) {
+    uint32_t bound;
+    {
+      const uint32_t v = warp_best[lane];
+      int larger = 0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t o = warp_best[j];
+        larger += (o > v || (o == v && j < lane)) ? 1 : 0;
+      }
+      const unsigned at = __ballot_sync(0xffffffffu, larger == p.top - 1);
+      bound = __shfl_sync(0xffffffffu, v, __ffs(at) - 1);
+    }
+    if (bound != 0 && mine >= bound) flagged[atomicAdd(&flagged_count, 1)] = tid;
+    __syncthreads();
+    const int rounds = (v1 - v0 + kThreads - 1) / kThreads;  // vectors of a thread, at most
+    const int n = flagged_count;
+    auto offer_candidate = [&](float value, int at) {
+      if (order_value(value) < bound) return;
+      const int slot = atomicAdd(&candidate_count, 1);
+      if (slot < kMaxCandidates) keys[slot] = order_key(value, at);
+    };
+    if (bound != 0) {
+      for (int item = tid; item < n * rounds; item += kThreads) {
+        const int v = v0 + flagged[item / rounds] + item % rounds * kThreads;
+        if (v < v1) {
+          float f[N];
+          L::unpack(__ldg(body + v), f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) offer_candidate(f[i], head + v * N + i);
+        }
+      }
+      if (at_head >= 0) offer_candidate(L::get(x + at_head), at_head);
+      if (at_tail >= 0) offer_candidate(L::get(x + at_tail), at_tail);
+    }
+    __syncthreads();
+    const int found = candidate_count;
+    if (bound != 0 && found <= kMaxCandidates) {
+      if (tid < found) {
+        const Key k = keys[tid];
+        int larger = 0;
+        for (int j = 0; j < found; ++j) larger += keys[j] > k ? 1 : 0;
+        if (larger < p.top) sorted[larger] = k;
+      }
+    } else {
+      // Every element once more; each warp keeps a descending list, one key per lane.
+      Key list = 0;
+      auto offer = [&](Key k) {
+        const Key last = shfl_key(list, 31);
+        unsigned want = __ballot_sync(0xffffffffu, k > last && (uint32_t)(k >> 32) >= bound);
+        while (want) {
+          const Key c = shfl_key(k, __ffs(want) - 1);
+          want &= want - 1;
+          const int at = __popc(__ballot_sync(0xffffffffu, list > c));
+          const Key up = __shfl_up_sync(0xffffffffu, list, 1);
+          list = lane < at ? list : (lane == at ? c : up);
+        }
+      };
+      for (int v = v0 + warp * 32; v < v1; v += kThreads) {
+        float f[N];
+        if (v + lane < v1) L::unpack(__ldg(body + v + lane), f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) offer(v + lane < v1 ? order_key(f[i], head + (v + lane) * N + i) : 0ull);
+      }
+      offer(at_head >= 0 ? order_key(L::get(x + at_head), at_head) : 0ull);
+      offer(at_tail >= 0 ? order_key(L::get(x + at_tail), at_tail) : 0ull);
+      keys[warp * 32 + lane] = list;
+      __syncthreads();
+      if (warp == 0) sorted[lane] = merge_lists(keys, kWarps, lane);
+    }
+  }
+  if (warp == 1) {
     Stats all = lane < kWarps ? warp_stats[lane] : empty_stats();
     all = warp_join(all);
-    int n = lane < kWarps ? warp_before[lane] : 0;
+    int sum = lane < kWarps ? warp_before[lane] : 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     st = all;
-    before = n;
+    before = sum;
+    if (csize == 1 && lane == 0) row_stats = st;
   }
+  __syncthreads();
   cluster_wait();
   if (csize > 1) {
-    if (warp == 0) {
-      Part *part = parts + crank;
-      if (lane == 0) {
-        store_cluster(in_first_cta(&part->st.m), __float_as_uint(st.m));
-        store_cluster(in_first_cta(&part->st.s), __float_as_uint(st.s));
-        store_cluster(in_first_cta(&part->st.u), __float_as_uint(st.u));
-        store_cluster(in_first_cta(&part->before), (uint32_t)before);
-      }
-      if (TOP) store_cluster(in_first_cta(&part->top[lane]), top_key);
+    Part *part = parts + crank;
+    if (tid == 32) {
+      store_cluster(in_first_cta(&part->st.m), __float_as_uint(st.m));
+      store_cluster(in_first_cta(&part->st.s), __float_as_uint(st.s));
+      store_cluster(in_first_cta(&part->st.u), __float_as_uint(st.u));
+      store_cluster(in_first_cta(&part->before), (uint32_t)before);
     }
+    if (TOP && tid < 32) store_cluster(in_first_cta(&part->top[tid]), sorted[tid]);
     __syncwarp();
     cluster_arrive();
     cluster_wait();
     if (crank != 0) return;
-    if (warp == 0) {
+    if (warp == 1) {
       st = lane < csize ? parts[lane].st : empty_stats();
       st = warp_join(st);
       before = lane < csize ? parts[lane].before : 0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      if (TOP)
-        for (int c = 1; c < csize; ++c) top_key = warp_merge(top_key, parts[c].top[lane], lane);
+      if (lane == 0) row_stats = st;
     }
+    __syncthreads();
   }
-  if (warp != 0) return;
   // With nothing but masked logits no token has any probability: every log
   // probability is -inf, the entropy 0. +inf or NaN among the logits make s,
   // and with it every result, NaN.
-  const bool none = st.m == -INFINITY && st.s == 0.0f;
-  const float log_s = none ? 0.0f : log2f(st.s) * kLn2;
-  auto log_p = [&](float v) { return none ? -INFINITY : (v - st.m) - log_s; };
-  if (lane == 0) {
+  const Stats r = row_stats;
+  const bool none = r.m == -INFINITY && r.s == 0.0f;
+  const float log_s = none ? 0.0f : log2f(r.s) * kLn2;
+  auto log_p = [&](float v) { return none ? -INFINITY : (v - r.m) - log_s; };
+  if (tid == 32) {
     if (p.logprobs) p.logprobs[row] = bad_target ? NAN : (given ? log_p(xt) : 0.0f);
-    if (p.entropy) p.entropy[row] = none ? 0.0f : log_s - st.u / st.s;
+    if (p.entropy) p.entropy[row] = none ? 0.0f : log_s - r.u / r.s;
     if (p.ranks) p.ranks[row] = given ? before : -1;
   }
-  if (TOP && lane < p.top) {
-    const int id = argmax_key_index(top_key);
-    p.top_ids[(size_t)row * p.top + lane] = id;
-    p.top_logprobs[(size_t)row * p.top + lane] = log_p(L::get(x + id));
+  if (TOP) {
+    // A key's place in the row: its place in its own list and the larger keys of the others.
+    const int list = warp, i = lane;  // kMaxCluster lists at most, one per warp
+    Key k = 0;
+    int place = i;
+    if (csize == 1) {
+      if (list == 0) k = sorted[i];
+    } else if (list < csize) {
+      k = parts[list].top[i];
+      if (k != 0)
+        for (int c = 0; c < csize; ++c)
+          if (c != list) place += larger_in(parts[c].top, k);
+    }
+    if (k != 0 && place < p.top) {
+      p.top_ids[(size_t)row * p.top + place] = argmax_key_index(k);
+      p.top_logprobs[(size_t)row * p.top + place] = log_p(argmax_key_value(k));
+    }
   }
 }
 
