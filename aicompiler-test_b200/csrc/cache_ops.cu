@@ -50,7 +50,8 @@ __device__ __forceinline__ uint32_t pack2(float2 v, __nv_bfloat16) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-constexpr int kCompactThreads = 128;
+constexpr int kCompactThreads = 64;
+constexpr int kHeads = 4;  // heads whose key and value a thread has in flight
 
 // Row i of the kept list moves from position p = keep[i] to position
 // t = first + i of the target pages. A key was stored rotated by its position,
@@ -96,20 +97,28 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const Compa
   const size_t a = (size_t)s * p.hkv * head + (size_t)(from % p.page_size) * vectors + c;
   const size_t b = (size_t)t * p.hkv * head + (size_t)(to % p.page_size) * vectors + c;
   uint4 *k = static_cast<uint4 *>(p.pools[2 * blockIdx.y]), *v = static_cast<uint4 *>(p.pools[2 * blockIdx.y + 1]);
-#pragma unroll 4
-  for (int h = 0; h < p.hkv; ++h) {
-    uint4 key = k[a + h * head];
-    const uint4 value = v[a + h * head];
-    if (turn) {
-      uint32_t *w = reinterpret_cast<uint32_t *>(&key);
+  for (int h0 = 0; h0 < p.hkv; h0 += kHeads) {
+    uint4 key[kHeads], value[kHeads];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack2(w[j], E());
-        w[j] = pack2(make_float2(fmaf(x.x, cs[j], x.y * sn[j]), fmaf(x.y, cs[j], -x.x * sn[j])), E());
+    for (int j = 0; j < kHeads; ++j)
+      if (h0 + j < p.hkv) {
+        key[j] = k[a + (h0 + j) * head];
+        value[j] = v[a + (h0 + j) * head];
       }
-    }
-    k[b + h * head] = key;
-    v[b + h * head] = value;
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j)
+      if (h0 + j < p.hkv) {
+        if (turn) {
+          uint32_t *w = reinterpret_cast<uint32_t *>(&key[j]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const float2 x = unpack2(w[n], E());
+            w[n] = pack2(make_float2(fmaf(x.x, cs[n], x.y * sn[n]), fmaf(x.y, cs[n], -x.x * sn[n])), E());
+          }
+        }
+        k[b + (h0 + j) * head] = key[j];
+        v[b + (h0 + j) * head] = value[j];
+      }
   }
 }
 

@@ -1,13 +1,13 @@
 // Token log probabilities, entropy, rank and top alternatives (logprobs.cuh).
 //
-// For a row x of V logits and m = max x, with
+// For a row x of V logits and a number m near its maximum, with
 //   s = sum e^(x - m),  u = sum e^(x - m) (x - m)
 // the log normaliser is m + log s, the target's log probability
 // (x_t - m) - log s and the entropy log s - u / s. One pass over the row keeps
 // (m, s, u) per thread, rescaled when the running maximum rises, and counts
 // the logits that come before the target (larger, or equal at a lower index).
-// u is summed about the maximum so that a peaked row's small entropy does not
-// come out as a difference of two large numbers.
+// u is summed about (nearly) the maximum so that a peaked row's small entropy
+// does not come out as a difference of two large numbers.
 //
 // The top alternatives come from the same read. Every thread keeps its largest
 // logit; the top-th largest of each warp's four best of these is reached by at
@@ -39,44 +39,87 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 using Key = unsigned long long;
 
+// kVec logits of a 16-byte vector: unpacked to fp32, their maximum (NaN only
+// if all are), and how many exceed (or reach) a threshold.
 template <typename T>
 struct Logit;
 template <>
 struct Logit<float> {
-  static constexpr int kVec = 4;  // elements of a 16-byte vector
+  static constexpr int kVec = 4;
   static __device__ __forceinline__ float get(const float *p) { return *p; }
-  static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[4]) {
+  static __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
     x[0] = __uint_as_float(v.x);
     x[1] = __uint_as_float(v.y);
     x[2] = __uint_as_float(v.z);
     x[3] = __uint_as_float(v.w);
   }
+  static __device__ __forceinline__ float largest(const uint4 &v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  template <bool REACH>
+  static __device__ __forceinline__ float above(const uint4 &v, float t) {
+    float x[4];
+    unpack(v, x);
+    float n = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += (REACH ? x[i] >= t : x[i] > t) ? 1.0f : 0.0f;
+    return n;
+  }
 };
-template <>
-struct Logit<__half> {
+// Two logits to a register: the maximum and the comparisons take them in pairs.
+template <typename H, typename H2>
+struct PairLogit {
   static constexpr int kVec = 8;
-  static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
-  static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
+  static __device__ __forceinline__ H2 pair(uint32_t w) { return *reinterpret_cast<const H2 *>(&w); }
+  static __device__ __forceinline__ float2 both(const H2 &h);
+  static __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = half2_bits_to_float2(w[i]);
+      const float2 f = both(pair(w[i]));
       x[2 * i] = f.x;
       x[2 * i + 1] = f.y;
     }
   }
+  static __device__ __forceinline__ float largest(const uint4 &v) {
+    const float2 f = both(__hmax2(__hmax2(pair(v.x), pair(v.y)), __hmax2(pair(v.z), pair(v.w))));
+    return fmaxf(f.x, f.y);
+  }
+  // t is a logit of this type: exact in it. The counts of a pair add up in the
+  // type itself, where they are whole numbers up to 4.
+  template <bool REACH>
+  static __device__ __forceinline__ float above(const uint4 &v, const H2 &t) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    H2 n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = REACH ? __hge2(pair(w[i]), t) : __hgt2(pair(w[i]), t);
+    const float2 f = both(__hadd2(__hadd2(n[0], n[1]), __hadd2(n[2], n[3])));
+    return f.x + f.y;
+  }
 };
 template <>
-struct Logit<__nv_bfloat16> {
-  static constexpr int kVec = 8;
+__device__ __forceinline__ float2 PairLogit<__half, __half2>::both(const __half2 &h) {
+  return __half22float2(h);
+}
+template <>
+__device__ __forceinline__ float2 PairLogit<__nv_bfloat16, __nv_bfloat162>::both(const __nv_bfloat162 &h) {
+  const uint32_t w = *reinterpret_cast<const uint32_t *>(&h);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+struct Logit<__half> : PairLogit<__half, __half2> {
+  static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
+  template <bool REACH>
+  static __device__ __forceinline__ float above(const uint4 &v, float t) {
+    return PairLogit::above<REACH>(v, __float2half2_rn(t));
+  }
+};
+template <>
+struct Logit<__nv_bfloat16> : PairLogit<__nv_bfloat16, __nv_bfloat162> {
   static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ void unpack(const uint4 &v, float (&x)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  template <bool REACH>
+  static __device__ __forceinline__ float above(const uint4 &v, float t) {
+    return PairLogit::above<REACH>(v, __float2bfloat162_rn(t));
   }
 };
 
@@ -86,22 +129,18 @@ struct Stats {
 };
 __device__ __forceinline__ Stats empty_stats() { return {-INFINITY, 0.0f, 0.0f}; }
 
-// The statistics of two disjoint parts together. A part without finite weight
-// (m = -inf: nothing but masked logits) leaves the other as it is.
-__device__ __forceinline__ Stats join(const Stats &a, const Stats &b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.u + b.u};
-  const float da = fmaxf(a.m - m, -1e30f), db = fmaxf(b.m - m, -1e30f);
-  const float fa = exp2f(da * kLog2e), fb = exp2f(db * kLog2e);
-  return {m, fmaf(a.s, fa, b.s * fb), fmaf(fmaf(a.s, da, a.u), fa, fmaf(b.s, db, b.u) * fb)};
+// The statistics about another maximum m >= a.m. A part without finite weight
+// (a.m = -inf: nothing but masked logits) has s = u = 0, or NaN.
+__device__ __forceinline__ void move_to(Stats &a, float m) {
+  if (m == a.m) return;
+  const float d = fmaxf(a.m - m, -1e30f), f = exp2f(d * kLog2e);
+  a.u = fmaf(a.s, d, a.u) * f;
+  a.s *= f;
+  a.m = m;
 }
-
 __device__ __forceinline__ Stats warp_join(Stats a) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
-                 __shfl_xor_sync(0xffffffffu, a.u, o)});
-  return a;
+  move_to(a, warp_max(a.m));
+  return {a.m, warp_sum(a.s), warp_sum(a.u)};
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 0 below the normal range
@@ -115,43 +154,86 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {  // NaN if eithe
   return y;
 }
 
-// N logits (index of the first: at) into the running statistics, the count
-// before the target and the thread's largest logit.
-template <int N, bool TOP>
-__device__ __forceinline__ void take(const float (&x)[N], int at, float xt, int target, Stats &st, int &before,
-                                     int &best_at) {
-  float mx = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-  if (mx > st.m) {
-    if (st.m != -INFINITY) {
-      const float d = fmaxf(st.m - mx, -1e30f), f = exp2f(d * kLog2e);
-      st.u = fmaf(st.s, d, st.u) * f;
-      st.s *= f;
+// A thread's pass over its logits. Four partial sums, so that successive
+// logits do not wait for one another.
+template <typename T>
+struct Pass {
+  using L = Logit<T>;
+  static constexpr int N = L::kVec;
+  float m = -INFINITY, s[4] = {}, u[4] = {};
+  float before = 0.0f;     // logits before the target: a whole number below 2^24
+  float best = -INFINITY;  // the largest logit, and the first index of the vector that holds it
+  int best_at = -1;
+
+  // The sums are about m, which follows the maximum only when it has risen by
+  // more than kSlack (weights of up to e^kSlack lose no precision): rescaling
+  // at every rise of any of a warp's 32 maxima cost a third of the time.
+  static constexpr float kSlack = 8.0f;
+  __device__ __forceinline__ void raise(float mx, int at) {
+    if (mx > best) {
+      best = mx;
+      best_at = at;
     }
-    st.m = mx;
-    if (TOP) best_at = at;
-  }
-  const float m = st.m == -INFINITY ? 0.0f : st.m;
+    if (mx > m + kSlack) {
+      if (m != -INFINITY) {
+        const float d = fmaxf(m - mx, -1e30f), f = exp2f(d * kLog2e);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < 4; ++i) {
+          u[i] = fmaf(s[i], d, u[i]) * f;
+          s[i] *= f;
+        }
+      }
+      m = mx;
+    }
+  }
+  __device__ __forceinline__ void weigh(float x, float about, int i) {
     // A masked logit (-inf) or one far below the maximum: 0 times a finite number.
-    const float d = max_or_nan(x[i] - m, -1e4f);
+    const float d = max_or_nan(x - about, -1e4f);
     const float e = exp2_fast(d * kLog2e);
-    st.s += e;
-    st.u = fmaf(e, d, st.u);
+    s[i & 3] += e;
+    u[i & 3] = fmaf(e, d, u[i & 3]);
   }
-  if (at + N <= target) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) before += x[i] >= xt ? 1 : 0;
-  } else if (at > target) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) before += x[i] > xt ? 1 : 0;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) before += (x[i] > xt || (x[i] == xt && at + i < target)) ? 1 : 0;
+  // One logit.
+  __device__ __forceinline__ void take(float x, int at, float xt, int target) {
+    raise(x, at);
+    weigh(x, m == -INFINITY ? 0.0f : m, 0);
+    before += (x > xt || (x == xt && at < target)) ? 1.0f : 0.0f;
   }
-}
+  // V vectors, `step` vectors apart, the first at index `at`.
+  template <int V>
+  __device__ __forceinline__ void take(const uint4 *raw, int at, int step, float xt, int target) {
+    float mx[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) mx[v] = L::largest(raw[v]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) raise(mx[v], at + v * step * N);
+    const float about = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float x[N];
+      L::unpack(raw[v], x);
+#pragma unroll
+      for (int i = 0; i < N; ++i) weigh(x[i], about, i);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int first = at + v * step * N;
+      if (first > target) {
+        before += L::template above<false>(raw[v], xt);
+      } else if (first + N <= target) {
+        before += L::template above<true>(raw[v], xt);
+      } else {
+        float x[N];
+        L::unpack(raw[v], x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) before += (x[i] > xt || (x[i] == xt && first + i < target)) ? 1.0f : 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ Stats stats() const {
+    return {m, (s[0] + s[1]) + (s[2] + s[3]), (u[0] + u[1]) + (u[2] + u[3])};
+  }
+};
 
 // Larger logits first, then lower indices; NaN counts as -inf, -0 as 0.
 __device__ __forceinline__ Key order_key(float x, int index) { return argmax_key(__fadd_rn(x, 0.0f), index); }
@@ -195,6 +277,9 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The address of a shared variable in the cluster's first CTA, and stores to it.
@@ -210,21 +295,12 @@ __device__ __forceinline__ void store_cluster(uint32_t at, Key v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
 
-// How many keys of a descending list of 32 (padded with 0) are larger than k.
-__device__ __forceinline__ int larger_in(const Key *list, Key k) {
-  int n = 0;
-#pragma unroll
-  for (int step = 16; step > 0; step >>= 1)
-    if (list[n + step - 1] > k) n += step;
-  return n + (list[n] > k ? 1 : 0);
-}
-
 constexpr int kWarpBest = 4;           // largest logits per warp that make the bound
 constexpr int kMaxCandidates = kThreads;
 
 // Grid (rows x cluster); the CTAs of a cluster share one row.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobsParams p) {
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const LogprobsParams p) {
   using L = Logit<T>;
   constexpr int N = L::kVec;
   static_assert(kWarps * kWarpBest == 32, "a warp ranks the CTA's best, one per lane");
@@ -240,15 +316,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int csize = (int)cluster_size(), crank = (int)cluster_rank(), row = blockIdx.x / csize;
-  cluster_arrive();  // waited for before the first store to another CTA's memory
+  if (csize > 1) cluster_arrive_relaxed();  // waited for before the first store to another CTA's memory
   const T *x = static_cast<const T *>(p.logits) + (long long)row * p.row_stride;
 
   const int target = p.targets != nullptr ? p.targets[row] : -1;
-  const bool bad_target = target < -1 || target >= p.vocab;
-  if (bad_target && tid == 0 && crank == 0) report_status(p.status, kStatusTokenRange, kWhereScore, target, row);
-  const bool given = target >= 0 && !bad_target;
-  const float xt = given ? L::get(x + target) : INFINITY;
-
   // This CTA's logits: whole vectors [v0, v1) but for the row's ends. The
   // first `head` logits of the row come before its first 16-byte boundary.
   const int misaligned = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
@@ -261,33 +332,43 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
   const int at_head = crank == 0 && tid < head ? tid : -1;
   const int at_tail = crank == csize - 1 && tid < tail ? head + vectors * N + tid : -1;
 
-  Stats st = empty_stats();
-  int before = 0;
-  int best_at = -1;  // first index of the vector that holds the thread's largest logit
-  if (at_head >= 0) {
-    const float one[1] = {L::get(x + at_head)};
-    take<1, TOP>(one, at_head, xt, target, st, before, best_at);
-  }
-  constexpr int kUnroll = 32 / N;
-  for (int v = v0 + tid; v < v1; v += kThreads * kUnroll) {
-    uint4 raw[kUnroll];
+  // The first vectors are on their way before the target's logit is waited for.
+  constexpr int kBatch = 2;
+  const int stride = kThreads * kBatch;
+  int v = v0 + tid;
+  uint4 raw[kBatch];
+  auto load = [&](int from) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      if (v + i * kThreads < v1) raw[i] = __ldg(body + v + i * kThreads);
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
-      if (v + i * kThreads < v1) {
-        float f[N];
-        L::unpack(raw[i], f);
-        take<N, TOP>(f, head + (v + i * kThreads) * N, xt, target, st, before, best_at);
-      }
-  }
-  if (at_tail >= 0) {
-    const float one[1] = {L::get(x + at_tail)};
-    take<1, TOP>(one, at_tail, xt, target, st, before, best_at);
-  }
+    for (int i = 0; i < kBatch; ++i) raw[i] = __ldg(body + from + i * kThreads);
+  };
+  const int full = v1 - (kBatch - 1) * kThreads;  // a whole batch starts below
+  if (v < full) load(v);
+  const bool given = target >= 0 && target < p.vocab;
+  const float xt = given ? L::get(x + target) : INFINITY;
 
-  const uint32_t mine = TOP && best_at >= 0 ? order_value(st.m) : 0u;  // 0: nothing above -inf
+  Pass<T> pass;
+  if (at_head >= 0) pass.take(L::get(x + at_head), at_head, xt, target);
+  while (v < full) {
+    uint4 now[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) now[i] = raw[i];
+    const int at = head + v * N;
+    v += stride;
+    if (v < full) load(v);
+    constexpr int kTogether = kBatch;
+#pragma unroll
+    for (int i = 0; i < kBatch; i += kTogether)
+      pass.template take<kTogether>(now + i, at + i * kThreads * N, kThreads, xt, target);
+  }
+  for (; v < v1; v += kThreads) {
+    const uint4 one = __ldg(body + v);
+    pass.template take<1>(&one, head + v * N, 0, xt, target);
+  }
+  if (at_tail >= 0) pass.take(L::get(x + at_tail), at_tail, xt, target);
+
+  Stats st = pass.stats();
+  int before = (int)pass.before;
+  const uint32_t mine = TOP && pass.best_at >= 0 ? order_value(pass.best) : 0u;  // 0: nothing above -inf
   {
     const Stats w = warp_join(st);
 #pragma unroll
@@ -333,13 +414,22 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
       if (slot < kMaxCandidates) keys[slot] = order_key(value, at);
     };
     if (bound != 0) {
-      for (int item = tid; item < n * rounds; item += kThreads) {
-        const int v = v0 + flagged[item / rounds] + item % rounds * kThreads;
-        if (v < v1) {
-          float f[N];
-          L::unpack(__ldg(body + v), f);
+      for (int item = tid; item < n * rounds; item += 2 * kThreads) {
+        int at[2];
+        uint4 again[2];
 #pragma unroll
-          for (int i = 0; i < N; ++i) offer_candidate(f[i], head + v * N + i);
+        for (int j = 0; j < 2; ++j) {
+          const int k = item + j * kThreads;
+          at[j] = k < n * rounds ? v0 + flagged[k / rounds] + k % rounds * kThreads : v1;
+          if (at[j] < v1) again[j] = __ldg(body + at[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (at[j] >= v1 || order_value(L::largest(again[j])) < bound) continue;
+          float f[N];
+          L::unpack(again[j], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) offer_candidate(f[i], head + at[j] * N + i);
         }
       }
       if (at_head >= 0) offer_candidate(L::get(x + at_head), at_head);
@@ -392,8 +482,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
     if (csize == 1 && lane == 0) row_stats = st;
   }
   __syncthreads();
-  cluster_wait();
   if (csize > 1) {
+    cluster_wait();
     Part *part = parts + crank;
     if (tid == 32) {
       store_cluster(in_first_cta(&part->st.m), __float_as_uint(st.m));
@@ -424,6 +514,8 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
   const float log_s = none ? 0.0f : log2f(r.s) * kLn2;
   auto log_p = [&](float v) { return none ? -INFINITY : (v - r.m) - log_s; };
   if (tid == 32) {
+    const bool bad_target = !given && target != -1;
+    if (bad_target) report_status(p.status, kStatusTokenRange, kWhereScore, target, row);
     if (p.logprobs) p.logprobs[row] = bad_target ? NAN : (given ? log_p(xt) : 0.0f);
     if (p.entropy) p.entropy[row] = none ? 0.0f : log_s - r.u / r.s;
     if (p.ranks) p.ranks[row] = given ? before : -1;
@@ -437,9 +529,16 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const Logprobs
       if (list == 0) k = sorted[i];
     } else if (list < csize) {
       k = parts[list].top[i];
-      if (k != 0)
-        for (int c = 0; c < csize; ++c)
-          if (c != list) place += larger_in(parts[c].top, k);
+      // Binary searches in all lists (padded with 0) side by side.
+      int n[kMaxCluster] = {};
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1)
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c)
+          if (c < csize && parts[c].top[n[c] + step - 1] > k) n[c] += step;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < csize && c != list) place += n[c] + (parts[c].top[n[c]] > k ? 1 : 0);
     }
     if (k != 0 && place < p.top) {
       p.top_ids[(size_t)row * p.top + place] = argmax_key_index(k);
