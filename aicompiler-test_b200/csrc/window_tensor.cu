@@ -1,0 +1,535 @@
+// Window attention of prompts on the tcgen05 tensor cores (head dimensions 64
+// and 128; see window_attention.cu for the other shapes and for decoding).
+//
+// A CTA holds two tiles of 128 tile rows (query row x head of one KV head) and
+// walks the visible keys 128 at a time: S_t = Q_t K^T and O_t += P_t V by
+// tcgen05.mma, S, P and O in tensor memory (P, in the storage type, over the
+// first half of its S). Four warps per tile are its softmax, one thread per
+// tile row: while one tile's exponentials are taken the other tile's products
+// run. Two warps each bring K and V in through the block table (16-byte
+// copies into 128-byte-swizzled rows: any page size), one thread issues the
+// products.
+//
+// The running maximum m of a row is only moved when it has risen by more than
+// kSlack (powers of two up to 2^kSlack lose nothing in P): O is rescaled in
+// tensor memory only then.
+//
+// P is rounded once to the storage type; the row sum l is taken before that.
+// Each output then carries independent errors of half a step per key, which
+// together stay below the rounding of the output itself.
+//
+// Values that are infinite or NaN in a step that some row does not wholly see
+// would reach that row as 0 x inf: such a step marks the tile, and the tile's
+// rows are computed again by plain loops.
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "window_device.cuh"
+
+namespace tmc {
+namespace window {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kKeys = 128;  // of a step
+constexpr int kSoftmaxWarps = 8;
+constexpr int kLoadWarps = 4;  // two for K, two for V
+constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kFlagRing = 4;  // steps whose missing-key flags are kept: more than the stages
+constexpr float kSlack = 8.0f;
+constexpr uint32_t kTmemColumns = 512;
+
+template <int D>
+struct TensorCfg {
+  static constexpr int kHalf = kKeys * 128;             // bytes of 64 columns of a 128-row tile
+  static constexpr int kTile = D / 64 * kHalf;          // one of K, V or a Q tile
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kSmem = 1024 + 2 * kTile + kStages * 2 * kTile;
+  static_assert(kStages < kFlagRing, "flags outlive their stage");
+};
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 consecutive 32-bit columns of this warp's lanes (one row per thread).
+__device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const float (&v)[32]) {
+  const uint32_t *r = reinterpret_cast<const uint32_t *>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Shared-memory matrix descriptors of tiles of 128-byte rows with 128-byte
+// swizzle (start address, strides in 16 bytes, version 1, layout 2).
+// K-major (Q, K: a row is an M or N index): 1024 bytes between groups of 8
+// rows; 32 bytes further is 16 elements further along K.
+__device__ __forceinline__ uint64_t k_major(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)1u << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 |
+         (uint64_t)2u << 61;
+}
+// N-major (V: a row is a K index, 64 N indices long): `half` bytes between
+// blocks of 64 N indices, 1024 bytes between groups of 8 K indices.
+__device__ __forceinline__ uint64_t n_major(uint32_t addr, uint32_t half) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)(half >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+// kind::f16 instruction: D fp32, M 128, N columns, A and B both fp16 or both bf16.
+template <typename E>
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_n_major) {
+  constexpr uint32_t type = sizeof(E) == 2 && std::is_same<E, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTileRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 0 below the normal range
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile of 128 rows.
+__device__ __forceinline__ int swizzled(int r, int c) {
+  return (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// Grid (splits x tile pairs, Hkv, sequences).
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const WindowAttentionParams p, int splits) {
+  using C = TensorCfg<D>;
+  constexpr int S = C::kStages;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char *sQ = base, *sK = base + 2 * C::kTile, *sV = sK + S * C::kTile;
+  __shared__ __align__(8) uint64_t q_full, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ uint32_t tmem_base;
+  __shared__ __align__(16) unsigned char bad_keys[kFlagRing][kKeys];  // keys of a step whose page is missing
+  __shared__ int bad_any[kFlagRing][2];
+  __shared__ int marked[2];  // the tile met an infinity or NaN beside masked pairs
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  const int s = blockIdx.z, h = blockIdx.y, split = blockIdx.x % splits;
+  const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
+  const int g = p.hq / p.hkv;
+  const int m0 = (int)(blockIdx.x / splits) * 2 * kTileRows, total = seq.rows * g;
+  if (m0 >= total) return;
+  const int tiles = m0 + kTileRows < total ? 2 : 1;
+  const int m_end = min(m0 + 2 * kTileRows, total);
+  const Visible vis = visible_keys(p, seq.first + m0 / g, seq.first + (m_end - 1) / g);
+  const int chunk = ((vis.count + splits - 1) / splits + kKeys - 1) / kKeys * kKeys;
+  const int v0 = min(vis.count, split * chunk), v1 = min(vis.count, v0 + chunk);
+  const int steps = (v1 - v0 + kKeys - 1) / kKeys;
+  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
+  if (steps == 0) {  // a split beyond the keys
+    const int m = m0 + tid;
+    if (m < m_end)
+      *partial_ml(p, slots, splits, split, ((long long)s * p.max_rows + m / g) * p.hq + h * g + m % g) =
+          make_float2(-INFINITY, 0.0f);
+    return;
+  }
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      mbar_init(&q_full, kSoftmaxWarps);
+      mbar_init(&drained, 1);
+      for (int i = 0; i < S; ++i) {
+        mbar_init(&k_full[i], 2);
+        mbar_init(&v_full[i], 2);
+        mbar_init(&k_empty[i], 1);
+        mbar_init(&v_empty[i], 1);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&s_full[t], 1);
+        mbar_init(&p_full[t], 4);
+        mbar_init(&o_full[t], 1);
+        marked[t] = 0;
+      }
+      fence_barrier_init();
+    }
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(kTmemColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_base;
+  auto gave_up = [&](int step) {
+    report_status(p.status, kStatusWaitTimeout, kWhereAttention, step, s);
+  };
+
+  if (warp < kSoftmaxWarps) {
+    // ---- softmax: one thread per tile row ----
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane, m = m0 + t * kTileRows + r;
+    const bool used = m < total;
+    const int row = used ? m / g : 0, head = h * g + (used ? m % g : 0), pos = seq.first + row;
+    {
+      const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const E *>(p.q) +
+                                                       (seq.start + row) * p.q_stride + (long long)head * D);
+      unsigned char *dst = sQ + t * C::kTile;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        *reinterpret_cast<uint4 *>(dst + swizzled(r, c)) = used ? q[c] : make_uint4(0u, 0u, 0u, 0u);
+      fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    }
+    const int t0 = min(m0 + t * kTileRows, total - 1), t1 = min(m0 + (t + 1) * kTileRows, total) - 1;
+    const int p_lo = seq.first + t0 / g, p_hi = seq.first + t1 / g;  // of the tile's rows
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + t * kKeys, o_at = tmem + lanes + 2 * kKeys + t * D;
+    const float scale = p.scale * kLog2e;
+    float m_run = -INFINITY, l_run[4] = {};
+    bool failed = false;
+    if (t < tiles) {
+      for (int j = 0; j < steps; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1))) {
+          if (lane == 0) gave_up(j);
+          failed = true;
+          break;
+        }
+        fence_after();
+        const int first = v0 + j * kKeys, last = min(first + kKeys, v1) - 1;
+        const int j0 = vis.key(first), j1 = vis.key(last);
+        bool whole = first + kKeys <= v1 && j1 <= p_lo && (j0 > p_hi - p.window || j1 < p.sinks);
+        if (!whole) {
+          const int st = j % S;
+          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / S) & 1))) {
+            if (lane == 0) gave_up(j);
+            failed = true;
+            break;
+          }
+          bool special = false;
+          const uint4 *v = reinterpret_cast<const uint4 *>(sV + st * C::kTile);
+#pragma unroll 4
+          for (int i = 0; i < C::kTile / 16 / 128; ++i) special |= any_special(v[r + 128 * i], exponent_mask(E()));
+          if (special) marked[t] = 1;
+        }
+        whole = whole && (bad_any[j % kFlagRing][0] | bad_any[j % kFlagRing][1]) == 0;
+        // Keys 32 c .. 32 c + 31 of the step that this row sees.
+        auto seen = [&](int c) {
+          uint32_t bits = 0;
+#pragma unroll 8
+          for (int i = 0; i < 32; ++i) {
+            const int v = first + c * 32 + i, k = vis.key(v);
+            const bool see = v < v1 && k <= pos && (pos - k < p.window || k < p.sinks) &&
+                             !bad_keys[j % kFlagRing][c * 32 + i];
+            bits |= see ? 1u << i : 0u;
+          }
+          return bits;
+        };
+        uint32_t mask[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mask[c] = seen(c);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float x[32];
+          tmem_load32(s_at + c * 32, x);
+          wait_ld();
+          if (whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, (mask[c] >> i) & 1 ? x[i] : -INFINITY);
+          }
+        }
+        mx *= scale;
+        const bool rise = mx > m_run + kSlack;
+        if (__any_sync(0xffffffffu, rise)) {
+          const float f = rise ? exp2_fast(m_run - mx) : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l_run[i] *= f;
+          if (rise) m_run = mx;
+          if (j > 0) {  // S of this step was issued after O's last product: O is complete
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float x[32];
+              tmem_load32(o_at + c * 32, x);
+              wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] *= f;
+              tmem_store32(o_at + c * 32, x);
+            }
+          }
+        }
+        const float about = m_run == -INFINITY ? 0.0f : m_run;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float x[32];
+          uint32_t w[16];
+          tmem_load32(s_at + c * 32, x);
+          wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = exp2_fast(fmaf(x[i], scale, -about));
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = (mask[c] >> i) & 1 ? x[i] : 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) l_run[i & 3] += x[i];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pack2(x[2 * i], x[2 * i + 1], E());
+          tmem_store16(s_at + c * 16, w);  // over columns of S that have been read
+        }
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!failed && !__all_sync(0xffffffffu, mbar_wait(&o_full[t], 0))) {
+        if (lane == 0) gave_up(steps);
+        failed = true;
+      }
+      fence_after();
+      // The tile's four warps agree on whether it was marked.
+      if (t == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+      else asm volatile("bar.sync 2, 128;" ::: "memory");
+      const long long slot = ((long long)s * p.max_rows + row) * p.hq + head;
+      if (!failed && marked[t] != 0) {
+        for (int i = 0; i < 32; ++i) {
+          const int mi = m0 + t * kTileRows + (warp & 3) * 32 + i;
+          if (mi >= total) break;
+          const int q_row = mi / g, q_head = h * g + mi % g;
+          float mm, ll, o[(D + 31) / 32];
+          slow_row<E, D>(p, seq, s, h, q_head, q_row, vis, v0, v1, mm, ll, o, lane);
+          const long long q_slot = ((long long)s * p.max_rows + q_row) * p.hq + q_head;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            const int d = lane + 32 * n;
+            if (splits > 1)
+              partial_acc(p, slots, split, q_slot)[d] = o[n];
+            else
+              store1(p.out, (seq.start + q_row) * p.out_stride + (long long)q_head * D + d,
+                     ll > 0.0f || ll != ll ? o[n] / ll : 0.0f, E());
+          }
+          if (splits > 1 && lane == 0) *partial_ml(p, slots, splits, split, q_slot) = make_float2(mm, ll);
+        }
+      } else if (!failed) {
+        const float l = (l_run[0] + l_run[1]) + (l_run[2] + l_run[3]);
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float x[32];
+          tmem_load32(o_at + c * 32, x);
+          wait_ld();
+          if (!used) continue;
+          if (splits > 1) {
+            float4 *o = reinterpret_cast<float4 *>(partial_acc(p, slots, split, slot) + c * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          } else {
+            uint4 *o = reinterpret_cast<uint4 *>(static_cast<E *>(p.out) + (seq.start + row) * p.out_stride +
+                                                 (long long)head * D + c * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[i] = make_uint4(pack2(x[8 * i] * inv, x[8 * i + 1] * inv, E()),
+                                pack2(x[8 * i + 2] * inv, x[8 * i + 3] * inv, E()),
+                                pack2(x[8 * i + 4] * inv, x[8 * i + 5] * inv, E()),
+                                pack2(x[8 * i + 6] * inv, x[8 * i + 7] * inv, E()));
+          }
+        }
+        if (used && splits > 1) *partial_ml(p, slots, splits, split, slot) = make_float2(m_run, l);
+      }
+    }
+  } else if (warp < kMmaWarp) {
+    // ---- loads: warps 0, 1 bring K, warps 2, 3 bring V, 64 keys of a step each ----
+    const int lw = warp - kSoftmaxWarps, half = lw & 1;
+    const bool value = lw >= 2;
+    const E *pool = static_cast<const E *>(value ? p.v_pool : p.k_pool);
+    unsigned char *tile = value ? sV : sK;
+    uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
+    auto find = [&](int j, int i) {
+      const int v = v0 + j * kKeys + half * 64 + i * 32 + lane;
+      return v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
+    };
+    KeyPlace next[2] = {find(0, 0), find(0, 1)};
+    for (int j = 0; j < steps; ++j) {
+      const int st = j % S;
+      long long at[2];
+      bool bad[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int v = v0 + j * kKeys + half * 64 + i * 32 + lane;
+        at[i] = v < v1 ? pool_row(p, next[i], h, s) : -1;
+        bad[i] = v < v1 && at[i] < 0;
+        if (j + 1 < steps) next[i] = find(j + 1, i);
+      }
+      if (j >= S && !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / S) - 1) & 1))) {
+        if (lane == 0) gave_up(j);
+        break;
+      }
+      if (!value) {
+        bad_keys[j % kFlagRing][half * 64 + lane] = bad[0];
+        bad_keys[j % kFlagRing][half * 64 + 32 + lane] = bad[1];
+        const int any = __any_sync(0xffffffffu, bad[0] || bad[1]);
+        if (lane == 0) bad_any[j % kFlagRing][half] = any;
+      }
+      const uint32_t dst = smem_u32(tile + st * C::kTile);
+      constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // rows that a warp copies at a time
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll 4
+        for (int n = 0; n < 32; n += kRows) {
+          const int r = n + lane / kChunks, c = lane % kChunks;
+          const long long from = __shfl_sync(0xffffffffu, at[i], r);
+          cp_async16(dst + swizzled(half * 64 + i * 32 + r, c), pool + (from < 0 ? 0 : from * D + c * 8),
+                     from < 0 ? 0 : 16);
+        }
+      cp_async_commit();
+      cp_async_wait<0>();
+      fence_async();  // what the copies wrote, before the products read it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[st]);
+    }
+  } else if (lane == 0) {
+    // ---- products ----
+    constexpr uint32_t kScores = instruction<E>(kKeys, false), kOutputs = instruction<E>(D, true);
+    bool ok = mbar_wait(&q_full, 0);
+    auto scores = [&](int t, int j) {
+      const uint32_t q = smem_u32(sQ + t * C::kTile), k = smem_u32(sK + (j % S) * C::kTile);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t off = (i / 4) * C::kHalf + (i % 4) * 32;
+        mma_smem(tmem + t * kKeys, k_major(q + off), k_major(k + off), kScores, i > 0);
+      }
+      commit(&s_full[t]);
+    };
+    ok = ok && mbar_wait(&k_full[0], 0);
+    fence_after();
+    if (ok) {
+      for (int t = 0; t < tiles; ++t) scores(t, 0);
+      commit(&k_empty[0]);
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      const int st = j % S;
+      ok = mbar_wait(&v_full[st], (j / S) & 1);
+      if (j + 1 < steps) ok = ok && mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1);
+      for (int t = 0; t < tiles && ok; ++t) {
+        ok = mbar_wait(&p_full[t], j & 1);
+        if (!ok) break;
+        fence_after();
+        const uint32_t v = smem_u32(sV + st * C::kTile);
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+          mma_tmem(tmem + 2 * kKeys + t * D, tmem + t * kKeys + i * 8, n_major(v + i * 16 * 128, C::kHalf), kOutputs,
+                   j > 0 || i > 0);
+        if (j + 1 < steps)
+          scores(t, j + 1);
+        else
+          commit(&o_full[t]);
+      }
+      if (!ok) break;
+      commit(&v_empty[st]);
+      if (j + 1 < steps) commit(&k_empty[(j + 1) % S]);
+    }
+    if (!ok) {
+      // Something never came: the products in flight end (a bounded wait) before the memory is given back.
+      gave_up(-1);
+      commit(&drained);
+      (void)mbar_wait(&drained, 0);
+    }
+  }
+  pdl_launch_dependents();
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns) : "memory");
+  }
+}
+
+template <typename E, int D>
+cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaStream_t stream, bool pdl) {
+  const auto kernel = window_tensor_kernel<E, D>;
+  {
+    static std::mutex mu;
+    static std::map<int, bool> done;  // by device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!done[dev]) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TensorCfg<D>::kSmem);
+      if (e != cudaSuccess) return e;
+      done[dev] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pairs * splits), p.hkv, p.sequences);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = TensorCfg<D>::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p, splits);
+}
+
+}  // namespace
+
+cudaError_t launch_window_tensor(const WindowAttentionParams &p, bool bf16, int pairs, int splits, cudaStream_t stream,
+                                 bool pdl) {
+  if (p.d == 64)
+    return bf16 ? launch<__nv_bfloat16, 64>(p, pairs, splits, stream, pdl) : launch<__half, 64>(p, pairs, splits, stream, pdl);
+  if (p.d == 128)
+    return bf16 ? launch<__nv_bfloat16, 128>(p, pairs, splits, stream, pdl)
+                : launch<__half, 128>(p, pairs, splits, stream, pdl);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace window
+}  // namespace tmc
