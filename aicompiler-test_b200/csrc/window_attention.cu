@@ -748,7 +748,8 @@ cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, i
     return cudaErrorInvalidValue;
   const long long g = p.hq / p.hkv;
   if ((long long)p.hkv * ((g + 15) / 16) > 65535 || (long long)p.max_rows * g > (1ll << 30) / kMaxOuter ||
-      (long long)p.sequences * p.max_rows > (1ll << 32) / p.hq)
+      (long long)p.sequences * p.max_rows > (1ll << 32) / p.hq ||
+      (long long)p.pool_pages * p.hkv > (1ll << 32) / p.page_size - 1)  // pool rows are counted in 32 bits
     return cudaErrorInvalidValue;
   WindowAttentionParams q = p;
   q.page_shift = -1;

@@ -6,9 +6,8 @@
 // tcgen05.mma, S, P and O in tensor memory (P, in the storage type, over the
 // first half of its S). Four warps per tile are its softmax, one thread per
 // tile row: while one tile's exponentials are taken the other tile's products
-// run. Two warps each bring K and V in through the block table (16-byte
-// copies into 128-byte-swizzled rows: any page size), one thread issues the
-// products.
+// run. Three warps bring K and V in through the block table (16-byte copies
+// into 128-byte-swizzled rows: any page size), one thread issues the products.
 //
 // The running maximum m of a row is only moved when it has risen by more than
 // kSlack (powers of two up to 2^kSlack lose nothing in P): O is rescaled in
@@ -34,7 +33,7 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kKeys = 128;  // of a step
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 4;  // two for K, two for V
+constexpr int kLoadWarps = 3;
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kFlagRing = 4;  // steps whose missing-key flags are kept: more than the stages
@@ -57,8 +56,8 @@ __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // 32 consecutive 32-bit columns of this warp's lanes (one row per thread).
-__device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
-  uint32_t *r = reinterpret_cast<uint32_t *>(v);
+__device__ __forceinline__ void tmem_load32(uint32_t at, float *v) {
+  uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -67,17 +66,18 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(at));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const float (&v)[32]) {
-  const uint32_t *r = reinterpret_cast<const uint32_t *>(v);
+__device__ __forceinline__ void tmem_load16(uint32_t at, float *v) {
+  uint32_t r[16];
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
@@ -130,6 +130,26 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 0 below the norma
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations at once.
+__device__ __forceinline__ void fma2(float &a, float &b, float scale, float add) {
+  asm("{\n\t.reg .b64 x, s, c;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+      "fma.rn.f32x2 x, x, s, c;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(scale), "f"(add));
+}
+__device__ __forceinline__ void add2(float2 &sum, float a, float b) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(sum.x), "+f"(sum.y)
+      : "f"(a), "f"(b));
+}
+// Bits [a, b) of 32.
+__device__ __forceinline__ uint32_t bits_between(int a, int b) {
+  a = max(a, 0);
+  b = min(b, 32);
+  return a < b ? (0xffffffffu >> (32 - (b - a))) << a : 0u;
 }
 
 // Byte offset of 16-byte chunk c of row r in a tile of 128 rows.
@@ -226,7 +246,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * kKeys, o_at = tmem + lanes + 2 * kKeys + t * D;
     const float scale = p.scale * kLog2e;
-    float m_run = -INFINITY, l_run[4] = {};
+    float m_run = -INFINITY;
+    float2 l_run[2] = {};
+    // What this row sees, as numbers of keys: all below `always` (the sinks,
+    // and keys of the run that are sinks), and [from, to) of the run.
+    const int always = vis.sinks + max(0, min(p.sinks, pos + 1) - vis.low);
+    const int from = vis.sinks + max(0, pos - p.window + 1 - vis.low);
+    const int to = min(vis.sinks + pos + 1 - vis.low, v1);
     bool failed = false;
     if (t < tiles) {
       for (int j = 0; j < steps; ++j) {
@@ -252,74 +278,70 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
           for (int i = 0; i < C::kTile / 16 / 128; ++i) special |= any_special(v[r + 128 * i], exponent_mask(E()));
           if (special) marked[t] = 1;
         }
-        whole = whole && (bad_any[j % kFlagRing][0] | bad_any[j % kFlagRing][1]) == 0;
-        // Keys 32 c .. 32 c + 31 of the step that this row sees.
-        auto seen = [&](int c) {
-          uint32_t bits = 0;
-#pragma unroll 8
-          for (int i = 0; i < 32; ++i) {
-            const int v = first + c * 32 + i, k = vis.key(v);
-            const bool see = v < v1 && k <= pos && (pos - k < p.window || k < p.sinks) &&
-                             !bad_keys[j % kFlagRing][c * 32 + i];
-            bits |= see ? 1u << i : 0u;
-          }
-          return bits;
-        };
-        uint32_t mask[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-        if (!whole) {
+        const bool missing = (bad_any[j % kFlagRing][0] | bad_any[j % kFlagRing][1]) != 0;
+        float x[kKeys];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mask[c] = seen(c);
-        }
-        float mx = -INFINITY;
+        for (int c = 0; c < 4; ++c) tmem_load32(s_at + c * 32, x + c * 32);
+        wait_ld();
+        if (!whole || missing) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x[32];
-          tmem_load32(s_at + c * 32, x);
-          wait_ld();
-          if (whole) {
+          for (int c = 0; c < 4; ++c) {
+            const int v = first + c * 32;
+            uint32_t bits = bits_between(0 - v, min(always, v1) - v) | bits_between(from - v, to - v);
+            if (missing)
+              for (int i = 0; i < 32; ++i)
+                if (bad_keys[j % kFlagRing][c * 32 + i]) bits &= ~(1u << i);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, (mask[c] >> i) & 1 ? x[i] : -INFINITY);
+            for (int i = 0; i < 32; ++i) x[c * 32 + i] = (bits >> i) & 1 ? x[c * 32 + i] : -INFINITY;
           }
         }
-        mx *= scale;
+        float mx;
+        {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = fmaxf(x[i], x[i + 8]);
+#pragma unroll
+          for (int i = 16; i < kKeys; i += 16)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) y[n] = fmaxf(y[n], fmaxf(x[i + n], x[i + n + 8]));
+          mx = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))) * scale;
+        }
         const bool rise = mx > m_run + kSlack;
         if (__any_sync(0xffffffffu, rise)) {
           const float f = rise ? exp2_fast(m_run - mx) : 1.0f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) l_run[i] *= f;
+          for (int i = 0; i < 2; ++i) {
+            l_run[i].x *= f;
+            l_run[i].y *= f;
+          }
           if (rise) m_run = mx;
           if (j > 0) {  // S of this step was issued after O's last product: O is complete
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float x[32];
-              tmem_load32(o_at + c * 32, x);
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_load16(o_at + c, o);
               wait_ld();
+              uint32_t w[16];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] *= f;
-              tmem_store32(o_at + c * 32, x);
+              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * f);
+              tmem_store16(o_at + c, w);
             }
           }
         }
-        const float about = m_run == -INFINITY ? 0.0f : m_run;
+        // A masked score (-inf) has weight 0; a row that has seen nothing yet has m = -inf.
+        const float about = m_run == -INFINITY ? 0.0f : -m_run;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float x[32];
           uint32_t w[16];
-          tmem_load32(s_at + c * 32, x);
-          wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = exp2_fast(fmaf(x[i], scale, -about));
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = (mask[c] >> i) & 1 ? x[i] : 0.0f;
+          for (int i = 0; i < 16; ++i) {
+            float &a = x[c * 32 + 2 * i], &b = x[c * 32 + 2 * i + 1];
+            fma2(a, b, scale, about);
+            a = exp2_fast(a);
+            b = exp2_fast(b);
+            add2(l_run[i & 1], a, b);
+            w[i] = pack2(a, b, E());
           }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) l_run[i & 3] += x[i];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pack2(x[2 * i], x[2 * i + 1], E());
           tmem_store16(s_at + c * 16, w);  // over columns of S that have been read
         }
         wait_st();
@@ -356,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
           if (splits > 1 && lane == 0) *partial_ml(p, slots, splits, split, q_slot) = make_float2(mm, ll);
         }
       } else if (!failed) {
-        const float l = (l_run[0] + l_run[1]) + (l_run[2] + l_run[3]);
+        const float l = (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -383,28 +405,28 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
       }
     }
   } else if (warp < kMmaWarp) {
-    // ---- loads: warps 0, 1 bring K, warps 2, 3 bring V, 64 keys of a step each ----
-    const int lw = warp - kSoftmaxWarps, half = lw & 1;
-    const bool value = lw >= 2;
-    const E *pool = static_cast<const E *>(value ? p.v_pool : p.k_pool);
-    unsigned char *tile = value ? sV : sK;
-    uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
-    auto find = [&](int j, int i) {
-      const int v = v0 + j * kKeys + half * 64 + i * 32 + lane;
-      return v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
+    // ---- loads: the halves (64 keys) of K and of V of every step are dealt out
+    // to the warps in the order in which they are needed ----
+    const int load = warp - kSoftmaxWarps;
+    const int jobs = 4 * steps;  // per step: K 0, K 1, V 0, V 1
+    auto find = [&](int job, int i) {
+      const int v = v0 + (job >> 2) * kKeys + (job & 1) * 64 + i * 32 + lane;
+      return job < jobs && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
     };
-    KeyPlace next[2] = {find(0, 0), find(0, 1)};
-    for (int j = 0; j < steps; ++j) {
-      const int st = j % S;
-      long long at[2];
+    KeyPlace next[2] = {find(load, 0), find(load, 1)};
+    for (int job = load; job < jobs; job += kLoadWarps) {
+      const int j = job >> 2, st = j % S, half = job & 1;
+      const bool value = (job & 2) != 0;
+      uint32_t at[2];  // pool rows: below 2^32 for 128-byte rows of one GPU's memory; 0xffffffff: none
       bool bad[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int v = v0 + j * kKeys + half * 64 + i * 32 + lane;
-        at[i] = v < v1 ? pool_row(p, next[i], h, s) : -1;
-        bad[i] = v < v1 && at[i] < 0;
-        if (j + 1 < steps) next[i] = find(j + 1, i);
+        at[i] = v < v1 ? (uint32_t)pool_row(p, next[i], h, s) : 0xffffffffu;
+        bad[i] = v < v1 && at[i] == 0xffffffffu;
+        next[i] = find(job + kLoadWarps, i);
       }
+      uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
       if (j >= S && !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / S) - 1) & 1))) {
         if (lane == 0) gave_up(j);
         break;
@@ -415,16 +437,17 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
         const int any = __any_sync(0xffffffffu, bad[0] || bad[1]);
         if (lane == 0) bad_any[j % kFlagRing][half] = any;
       }
-      const uint32_t dst = smem_u32(tile + st * C::kTile);
       constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // rows that a warp copies at a time
+      const char *pool = static_cast<const char *>(value ? p.v_pool : p.k_pool) + (lane % kChunks) * 16;
+      const uint32_t dst = smem_u32((value ? sV : sK) + st * C::kTile) + half * 64 * 128;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-#pragma unroll 4
+#pragma unroll 8
         for (int n = 0; n < 32; n += kRows) {
           const int r = n + lane / kChunks, c = lane % kChunks;
-          const long long from = __shfl_sync(0xffffffffu, at[i], r);
-          cp_async16(dst + swizzled(half * 64 + i * 32 + r, c), pool + (from < 0 ? 0 : from * D + c * 8),
-                     from < 0 ? 0 : 16);
+          const uint32_t row = __shfl_sync(0xffffffffu, at[i], r);
+          const bool there = row != 0xffffffffu;
+          cp_async16(dst + swizzled(i * 32 + r, c), pool + (size_t)(there ? row : 0u) * (D * 2), there ? 16 : 0);
         }
       cp_async_commit();
       cp_async_wait<0>();
