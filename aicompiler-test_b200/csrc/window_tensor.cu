@@ -6,8 +6,10 @@
 // tcgen05.mma, S, P and O in tensor memory (P, in the storage type, over the
 // first half of its S). Four warps per tile are its softmax, one thread per
 // tile row: while one tile's exponentials are taken the other tile's products
-// run. Three warps bring K and V in through the block table (16-byte copies
-// into 128-byte-swizzled rows: any page size), one thread issues the products.
+// run. K and V come in through the block table: pages of whole groups of 16
+// positions as TMA boxes (the key numbering starts on a group then, and what
+// no row sees of a group is zeroed in V), other page sizes as 16-byte copies
+// by three warps. One thread issues the products.
 //
 // The running maximum m of a row is only moved when it has risen by more than
 // kSlack (powers of two up to 2^kSlack lose nothing in P): O is rescaled in
@@ -24,6 +26,7 @@
 #include <mutex>
 #include <utility>
 
+#include "gemm.cuh"
 #include "window_device.cuh"
 
 namespace tmc {
@@ -33,7 +36,8 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kKeys = 128;  // of a step
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 3;
+constexpr int kLoadWarps = 3;  // with boxes: one for K, one for V
+constexpr int kBox = 16;       // positions of a box
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kFlagRing = 4;  // steps whose missing-key flags are kept: more than the stages
@@ -157,15 +161,17 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   return (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// Grid (splits x tile pairs, Hkv, sequences).
-template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const WindowAttentionParams p, int splits) {
+// Grid (splits x tile pairs, Hkv, sequences). BOXES: K and V by TMA boxes.
+template <typename E, int D, bool BOXES>
+__global__ void __launch_bounds__(kThreads, 1)
+    window_tensor_kernel(const WindowAttentionParams p, int splits, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map) {
   using C = TensorCfg<D>;
   constexpr int S = C::kStages;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char *sQ = base, *sK = base + 2 * C::kTile, *sV = sK + S * C::kTile;
-  __shared__ __align__(8) uint64_t q_full, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ __align__(8) uint64_t q_full, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2], o_full[2], drained, v_landed;
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) unsigned char bad_keys[kFlagRing][kKeys];  // keys of a step whose page is missing
   __shared__ int bad_any[kFlagRing][2];
@@ -180,7 +186,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
   if (m0 >= total) return;
   const int tiles = m0 + kTileRows < total ? 2 : 1;
   const int m_end = min(m0 + 2 * kTileRows, total);
-  const Visible vis = visible_keys(p, seq.first + m0 / g, seq.first + (m_end - 1) / g);
+  const int p_last = seq.first + (m_end - 1) / g;
+  Visible vis = visible_keys(p, seq.first + m0 / g, p_last);
+  const int low = vis.low;  // keys below, but for the sinks, are seen by no row
+  if (BOXES) {  // both parts start and the first ends on a group
+    vis.low = low / kBox * kBox;
+    vis.sinks = min((min(p.sinks, vis.low) + kBox - 1) / kBox * kBox, vis.low);
+    vis.count = vis.sinks + p_last + 1 - vis.low;
+  }
   const int chunk = ((vis.count + splits - 1) / splits + kKeys - 1) / kKeys * kKeys;
   const int v0 = min(vis.count, split * chunk), v1 = min(vis.count, v0 + chunk);
   const int steps = (v1 - v0 + kKeys - 1) / kKeys;
@@ -197,9 +210,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
     if (lane == 0) {
       mbar_init(&q_full, kSoftmaxWarps);
       mbar_init(&drained, 1);
+      mbar_init(&v_landed, 1);
       for (int i = 0; i < S; ++i) {
-        mbar_init(&k_full[i], 2);
-        mbar_init(&v_full[i], 2);
+        mbar_init(&k_full[i], BOXES ? 1 : 2);
+        mbar_init(&v_full[i], BOXES ? 1 : 2);
         mbar_init(&k_empty[i], 1);
         mbar_init(&v_empty[i], 1);
       }
@@ -250,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
     float2 l_run[2] = {};
     // What this row sees, as numbers of keys: all below `always` (the sinks,
     // and keys of the run that are sinks), and [from, to) of the run.
-    const int always = vis.sinks + max(0, min(p.sinks, pos + 1) - vis.low);
+    const int always = p.sinks < vis.low ? p.sinks : vis.sinks + max(0, min(p.sinks, pos + 1) - vis.low);
     const int from = vis.sinks + max(0, pos - p.window + 1 - vis.low);
     const int to = min(vis.sinks + pos + 1 - vis.low, v1);
     bool failed = false;
@@ -404,7 +418,72 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
         if (used && splits > 1) *partial_ml(p, slots, splits, split, slot) = make_float2(m_run, l);
       }
     }
-  } else if (warp < kMmaWarp) {
+  } else if (BOXES && warp < kMmaWarp) {
+    // ---- loads by boxes: a warp for K, a warp for V, lane i < 8 takes group i of a step ----
+    const int load = warp - kSoftmaxWarps;
+    const bool value = load == 1;
+    auto find = [&](int j) {
+      const int v = v0 + j * kKeys + lane * kBox;
+      return lane < kKeys / kBox && j < steps && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
+    };
+    KeyPlace next = find(0);
+    uint32_t edges = 0;  // steps whose V rows were cleaned: the phase of v_landed
+    for (int j = 0; j < steps && load < 2; ++j) {
+      const int st = j % S, first = v0 + j * kKeys;
+      const bool here = lane < kKeys / kBox && first + lane * kBox < v1;
+      const long long row = here ? pool_row(p, next, h, s) : -1;
+      const unsigned bad = __ballot_sync(0xffffffffu, here && row < 0);
+      const int boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
+      next = find(j + 1);
+      uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
+      if (j >= S && !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / S) - 1) & 1))) {
+        if (lane == 0) gave_up(j);
+        break;
+      }
+      // V rows that no row of the tiles sees (outside the window's union, or
+      // of a missing page) hold anything: zeros in their place.
+      bool hide[kKeys / 32];
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < kKeys / 32; ++i) {
+        const int v = first + i * 32 + lane, k = vis.key(v);
+        hide[i] = v >= v1 || (k < low && k >= p.sinks) || ((bad >> ((i * 32 + lane) / kBox)) & 1);
+        any |= hide[i];
+      }
+      const bool edge = __any_sync(0xffffffffu, any) && value;
+      if (!value) {
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i)
+          bad_keys[j % kFlagRing][i * 32 + lane] = (bad >> ((i * 32 + lane) / kBox)) & 1;
+        if (lane < 2) bad_any[j % kFlagRing][lane] = bad != 0;
+        __syncwarp();
+      }
+      uint64_t *bar = edge ? &v_landed : &full[st];
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)boxes * kBox * D * 2);
+      __syncwarp();
+      unsigned char *dst = (value ? sV : sK) + st * C::kTile;
+      if (row >= 0) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_2d(dst + c * C::kHalf + lane * kBox * 128, value ? &v_map : &k_map, c * 64, (int)row, bar);
+      }
+      if (edge) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&v_landed, edges & 1))) {
+          if (lane == 0) gave_up(j);
+          break;
+        }
+        ++edges;
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i)
+          if (hide[i])
+            for (int c = 0; c < D / 8; ++c)
+              *reinterpret_cast<uint4 *>(dst + swizzled(i * 32 + lane, c)) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
+      }
+    }
+  } else if (!BOXES && warp < kMmaWarp) {
     // ---- loads: the halves (64 keys) of K and of V of every step are dealt out
     // to the warps in the order in which they are needed ----
     const int load = warp - kSoftmaxWarps;
@@ -513,9 +592,16 @@ __global__ void __launch_bounds__(kThreads, 1) window_tensor_kernel(const Window
   }
 }
 
-template <typename E, int D>
+template <typename E, int D, bool BOXES>
 cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaStream_t stream, bool pdl) {
-  const auto kernel = window_tensor_kernel<E, D>;
+  const auto kernel = window_tensor_kernel<E, D, BOXES>;
+  CUtensorMap k_map{}, v_map{};
+  if (BOXES) {  // 16-bit elements of either kind: boxes only move them
+    const uint64_t rows = (uint64_t)p.pool_pages * p.hkv * p.page_size;
+    cudaError_t e = make_tensor_map_f16(&k_map, p.k_pool, rows, D, kBox);
+    if (e == cudaSuccess) e = make_tensor_map_f16(&v_map, p.v_pool, rows, D, kBox);
+    if (e != cudaSuccess) return e;
+  }
   {
     static std::mutex mu;
     static std::map<int, bool> done;  // by device
@@ -539,19 +625,25 @@ cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaSt
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p, splits);
+  return cudaLaunchKernelEx(&cfg, kernel, p, splits, k_map, v_map);
+}
+
+template <typename E>
+cudaError_t dispatch(const WindowAttentionParams &p, int pairs, int splits, cudaStream_t stream, bool pdl) {
+  const bool boxes = p.page_size % kBox == 0 && (long long)p.pool_pages * p.hkv <= 0x7fffffffll / p.page_size;
+  if (p.d == 64)
+    return boxes ? launch<E, 64, true>(p, pairs, splits, stream, pdl) : launch<E, 64, false>(p, pairs, splits, stream, pdl);
+  if (p.d == 128)
+    return boxes ? launch<E, 128, true>(p, pairs, splits, stream, pdl)
+                 : launch<E, 128, false>(p, pairs, splits, stream, pdl);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
 cudaError_t launch_window_tensor(const WindowAttentionParams &p, bool bf16, int pairs, int splits, cudaStream_t stream,
                                  bool pdl) {
-  if (p.d == 64)
-    return bf16 ? launch<__nv_bfloat16, 64>(p, pairs, splits, stream, pdl) : launch<__half, 64>(p, pairs, splits, stream, pdl);
-  if (p.d == 128)
-    return bf16 ? launch<__nv_bfloat16, 128>(p, pairs, splits, stream, pdl)
-                : launch<__half, 128>(p, pairs, splits, stream, pdl);
-  return cudaErrorInvalidValue;
+  return bf16 ? dispatch<__nv_bfloat16>(p, pairs, splits, stream, pdl) : dispatch<__half>(p, pairs, splits, stream, pdl);
 }
 
 }  // namespace window
