@@ -136,19 +136,6 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 0 below the norma
   return y;
 }
 
-// Two fp32 operations at once.
-__device__ __forceinline__ void fma2(float &a, float &b, float scale, float add) {
-  asm("{\n\t.reg .b64 x, s, c;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 s, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
-      "fma.rn.f32x2 x, x, s, c;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(a), "+f"(b)
-      : "f"(scale), "f"(add));
-}
-__device__ __forceinline__ void add2(float2 &sum, float a, float b) {
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
-      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-      : "+f"(sum.x), "+f"(sum.y)
-      : "f"(a), "f"(b));
-}
 // Bits [a, b) of 32.
 __device__ __forceinline__ uint32_t bits_between(int a, int b) {
   a = max(a, 0);
@@ -179,10 +166,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
-  const int s = blockIdx.z, h = blockIdx.y, split = blockIdx.x % splits;
+  const int s = blockIdx.z, h = blockIdx.y, split = (gridDim.x - 1 - blockIdx.x) % splits;
   const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
   const int g = p.hq / p.hkv;
-  const int m0 = (int)(blockIdx.x / splits) * 2 * kTileRows, total = seq.rows * g;
+  // The last rows see the most keys: their tiles start first.
+  const int m0 = (int)((gridDim.x - 1 - blockIdx.x) / splits) * 2 * kTileRows, total = seq.rows * g;
   if (m0 >= total) return;
   const int tiles = m0 + kTileRows < total ? 2 : 1;
   const int m_end = min(m0 + 2 * kTileRows, total);
@@ -349,12 +337,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float &a = x[c * 32 + 2 * i], &b = x[c * 32 + 2 * i + 1];
-            fma2(a, b, scale, about);
-            a = exp2_fast(a);
-            b = exp2_fast(b);
-            add2(l_run[i & 1], a, b);
-            w[i] = pack2(a, b, E());
+            const float a = x[c * 32 + 2 * i], b = x[c * 32 + 2 * i + 1];
+            const float2 t = __ffma2_rn(make_float2(a, b), make_float2(scale, scale), make_float2(about, about));
+            const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+            l_run[i & 1] = __fadd2_rn(l_run[i & 1], e);
+            w[i] = pack2(e.x, e.y, E());
           }
           tmem_store16(s_at + c * 16, w);  // over columns of S that have been read
         }
