@@ -28,9 +28,6 @@ namespace {
 
 using namespace window;
 
-#ifndef TMC_TK
-#define TMC_TK 256
-#endif
 constexpr int kMaxCluster = 8;    // CTAs of a decode cluster
 constexpr int kDecodePerSm = 3;  // decode CTAs that an SM holds
 constexpr int kMaxOuter = 32;    // splits that meet through the workspace
@@ -554,42 +551,59 @@ __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
 
 // ---- joining splits ----------------------------------------------------------------------
 
-// One thread per element, D of them per (sequence, row, head): out =
-// sum_i w_i acc_i / sum_i w_i l_i, w_i = 2^(m_i - max m). All partial sums are
-// read before they are needed; those of empty splits hold nothing and are
-// left out by their weight.
-template <typename E>
-__global__ void __launch_bounds__(128) window_join_kernel(const WindowAttentionParams p, int splits) {
-  const int lane = threadIdx.x & 31;
+// out = sum_i w_i acc_i / sum_i w_i l_i with w_i = 2^(m_i - max m). Grid (rows
+// of a sequence, sequences, head groups); a thread owns four elements of one
+// head. Empty splits hold no sums: their weight is 0 and they are left out.
+// (A thread per element that found its place by divisions took 33 us where
+// this takes 5: 256 rows of 32 heads, three splits.)
+constexpr int kJoinThreads = 128;
+template <typename E, int D>
+__global__ void __launch_bounds__(kJoinThreads) window_join_kernel(const WindowAttentionParams p, int splits) {
+  constexpr int kHeads = kJoinThreads * 4 / D;  // of a group
+  __shared__ float2 parts[kHeads][kMaxOuter];   // (m, l)
   pdl_wait();
   pdl_launch_dependents();
-  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-  const int lanes = p.d < 32 ? 32 : p.d;  // threads per slot: whole warps
-  const long long index = (long long)blockIdx.x * 128 + threadIdx.x;
-  const long long slot = index / lanes;
-  const int d = (int)(index % lanes);
-  if (slot >= slots) return;
-  const int head = (int)(slot % p.hq), row = (int)(slot / p.hq % p.max_rows), s = (int)(slot / p.hq / p.max_rows);
-  float2 ml = lane < splits ? __ldcg(partial_ml(p, slots, splits, lane, slot)) : make_float2(-INFINITY, 0.0f);
-  float x[kMaxOuter];
-  const float *acc = partial_acc(p, slots, 0, slot) + (d < p.d ? d : 0);
-#pragma unroll
-  for (int i = 0; i < kMaxOuter; ++i)
-    if (i < splits) x[i] = __ldcg(acc + i * slots * p.d);
+  const int row = blockIdx.x, s = blockIdx.y, h0 = blockIdx.z * kHeads, tid = threadIdx.x;
+  const int heads = min(kHeads, p.hq - h0);
   const Sequence seq = load_sequence(p, s, false);
+  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
+  const long long slot0 = ((long long)s * p.max_rows + row) * p.hq + h0;
   if (row >= seq.rows) return;
-  const float m = warp_max(ml.x);
-  const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - m);
-  // A state without weight counts by its sum alone: 0, or NaN.
-  const float l = warp_sum(ml.x == -INFINITY ? ml.y : ml.y * w);
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-  float o = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kMaxOuter; ++i) {
-    const float wi = __shfl_sync(0xffffffffu, w, i);
-    if (i < splits && wi != 0.0f) o = fmaf(x[i], wi, o);
+  for (int i = tid; i < heads * kMaxOuter; i += kJoinThreads) {
+    const int h = i / kMaxOuter, n = i % kMaxOuter;
+    if (n < splits) parts[h][n] = __ldcg(partial_ml(p, slots, splits, n, slot0 + h));
   }
-  if (d < p.d) store1(p.out, (seq.start + row) * p.out_stride + (long long)head * p.d + d, o * inv, E());
+  const int h = tid / (D / 4), d = tid % (D / 4) * 4;
+  const bool own = h < heads;
+  const float *acc = partial_acc(p, slots, 0, slot0 + (own ? h : 0)) + d;
+  constexpr int kBatch = 8;
+  float4 x[kBatch];
+  auto load = [&](int n0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (n0 + i < splits) x[i] = __ldcg(reinterpret_cast<const float4 *>(acc + (n0 + i) * slots * D));
+  };
+  load(0);
+  __syncthreads();
+  if (!own) return;
+  float m = -INFINITY, l = 0.0f;
+  for (int n = 0; n < splits; ++n) m = fmaxf(m, parts[h][n].x);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int n0 = 0; n0 < splits; n0 += kBatch) {
+    if (n0 > 0) load(n0);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (n0 + i >= splits) break;
+      const float2 ml = parts[h][n0 + i];
+      if (ml.x == -INFINITY)
+        l += ml.y;  // nothing but its sum counts: 0, or NaN
+      else
+        join_part(ml, x[i], m, l, o);
+    }
+  }
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  *reinterpret_cast<uint2 *>(static_cast<E *>(p.out) + (seq.start + row) * p.out_stride + (long long)(h0 + h) * D + d) =
+      make_uint2(pack2(o.x * inv, o.y * inv, E()), pack2(o.z * inv, o.w * inv, E()));
 }
 
 // ---- launches ----------------------------------------------------------------------------
@@ -613,7 +627,11 @@ Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long ke
   const long long ctas = (long long)sequences * hkv * plan.tiles;
   const long long slots = (plan.decode ? kDecodePerSm : plan.tensor ? 1 : 2) * num_sms;  // CTAs that run at the same time
   if (plan.tensor) {
-    while (plan.outer < kMaxOuter && ctas * (plan.outer + 1) <= slots && keys >= TMC_TK * (plan.outer + 1)) ++plan.outer;
+    const long long steps = (keys + 127) / 128;
+    long long splits = slots / ctas;
+    splits = splits < 1 ? 1 : splits < kMaxOuter ? splits : kMaxOuter;
+    if (splits > steps) splits = steps;
+    plan.outer = (int)((steps + (steps + splits - 1) / splits - 1) / ((steps + splits - 1) / splits));  // none empty
     return plan;
   }
   if (!plan.decode) {
@@ -709,13 +727,13 @@ cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t str
     e = cudaLaunchKernelEx(&cfg, kernel, p, plan.outer);
   }
   if (e != cudaSuccess || plan.outer == 1) return e;
-  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-  cfg.gridDim = dim3((unsigned)((slots * (D < 32 ? 32 : D) + 127) / 128));
-  cfg.blockDim = dim3(128);
+  constexpr int kHeads = kJoinThreads * 4 / D;
+  cfg.gridDim = dim3(p.max_rows, p.sequences, (p.hq + kHeads - 1) / kHeads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 0;
   add_pdl();
-  return cudaLaunchKernelEx(&cfg, window_join_kernel<E>, p, plan.outer);
+  return cudaLaunchKernelEx(&cfg, window_join_kernel<E, D>, p, plan.outer);
 }
 
 template <typename E>
@@ -747,7 +765,7 @@ cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, i
       p.window <= 0 || p.sinks < 0 || p.q_stride % 8 != 0 || p.out_stride % 8 != 0)
     return cudaErrorInvalidValue;
   const long long g = p.hq / p.hkv;
-  if ((long long)p.hkv * ((g + 15) / 16) > 65535 || (long long)p.max_rows * g > (1ll << 30) / kMaxOuter ||
+  if ((long long)p.hkv * ((g + 15) / 16) > 65535 || p.hq > 65535 || (long long)p.max_rows * g > (1ll << 30) / kMaxOuter ||
       (long long)p.sequences * p.max_rows > (1ll << 32) / p.hq ||
       (long long)p.pool_pages * p.hkv > (1ll << 32) / p.page_size - 1)  // pool rows are counted in 32 bits
     return cudaErrorInvalidValue;
