@@ -241,13 +241,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, m = m0 + t * kTileRows + r;
     const bool used = m < total;
     const int row = used ? m / g : 0, head = h * g + (used ? m % g : 0), pos = seq.first + row;
+    // Rows go to and from shared memory by whole warps, a few rows at a time
+    // (each thread its own row: 4 us more per CTA for Q, 2 for the results).
+    constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows at a time
+    unsigned char *own_rows = sQ + t * C::kTile;
+    const int r0 = (warp & 3) * 32;
     {
-      const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const E *>(p.q) +
-                                                       (seq.start + row) * p.q_stride + (long long)head * D);
-      unsigned char *dst = sQ + t * C::kTile;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        *reinterpret_cast<uint4 *>(dst + swizzled(r, c)) = used ? q[c] : make_uint4(0u, 0u, 0u, 0u);
+      const long long at = used ? (seq.start + row) * p.q_stride + (long long)head * D : -1;
+#pragma unroll 8
+      for (int n = 0; n < 32; n += kRows) {
+        const int i = n + lane / kChunks, c = lane % kChunks;
+        const long long from = __shfl_sync(0xffffffffu, at, i);
+        cp_async16(smem_u32(own_rows + swizzled(r0 + i, c)), static_cast<const E *>(p.q) + (from < 0 ? 0 : from + c * 8),
+                   from < 0 ? 0 : 16);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
       fence_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
@@ -389,26 +398,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else if (!failed) {
         const float l = (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float x[32];
-          tmem_load32(o_at + c * 32, x);
-          wait_ld();
-          if (!used) continue;
-          if (splits > 1) {
-            float4 *o = reinterpret_cast<float4 *>(partial_acc(p, slots, split, slot) + c * 32);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          } else {
-            uint4 *o = reinterpret_cast<uint4 *>(static_cast<E *>(p.out) + (seq.start + row) * p.out_stride +
-                                                 (long long)head * D + c * 32);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              o[i] = make_uint4(pack2(x[8 * i] * inv, x[8 * i + 1] * inv, E()),
-                                pack2(x[8 * i + 2] * inv, x[8 * i + 3] * inv, E()),
-                                pack2(x[8 * i + 4] * inv, x[8 * i + 5] * inv, E()),
-                                pack2(x[8 * i + 6] * inv, x[8 * i + 7] * inv, E()));
+        // Q has been read: its place takes the results, 256-byte (D 64: 128-byte) pieces of each row.
+        const long long row_at = !used ? -1 : splits > 1 ? (split * slots + slot) * D : (seq.start + row) * p.out_stride + (long long)head * D;
+        auto hand_out = [&](char *to, int size, int bytes_before) {  // the warp's 32 rows, chunks in order
+          __syncwarp();
+#pragma unroll 4
+          for (int n = 0; n < 32; n += kRows) {
+            const int i = n + lane / kChunks, c = lane % kChunks;
+            const long long dst = __shfl_sync(0xffffffffu, row_at, i);
+            if (dst >= 0)
+              *reinterpret_cast<uint4 *>(to + dst * size + bytes_before + c * 16) =
+                  *reinterpret_cast<const uint4 *>(own_rows + swizzled(r0 + i, c));
           }
+          __syncwarp();
+        };
+        if (splits > 1) {
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) {  // D / 2 fp32 columns fill a row's place
+#pragma unroll 1
+            for (int c = 0; c < D / 2; c += 16) {
+              float x[16];
+              tmem_load16(o_at + part * (D / 2) + c, x);
+              wait_ld();
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4 *>(own_rows + swizzled(r, c / 4 + i)) =
+                    make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            }
+            hand_out(static_cast<char *>(p.workspace), 4, part * D * 2);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float x[16];
+            tmem_load16(o_at + c, x);
+            wait_ld();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<uint4 *>(own_rows + swizzled(r, c / 8 + i)) =
+                  make_uint4(pack2(x[8 * i] * inv, x[8 * i + 1] * inv, E()),
+                             pack2(x[8 * i + 2] * inv, x[8 * i + 3] * inv, E()),
+                             pack2(x[8 * i + 4] * inv, x[8 * i + 5] * inv, E()),
+                             pack2(x[8 * i + 6] * inv, x[8 * i + 7] * inv, E()));
+          }
+          hand_out(static_cast<char *>(p.out), 2, 0);
         }
         if (used && splits > 1) *partial_ml(p, slots, splits, split, slot) = make_float2(m_run, l);
       }
