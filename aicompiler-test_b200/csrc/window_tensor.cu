@@ -11,9 +11,10 @@
 // no row sees of a group is zeroed in V), other page sizes as 16-byte copies
 // by three warps. One thread issues the products.
 //
-// The running maximum m of a row is only moved when it has risen by more than
-// kSlack (powers of two up to 2^kSlack lose nothing in P): O is rescaled in
-// tensor memory only then.
+// Weights are 2^(s - m) about a number m per row that only moves, to the
+// maximum seen, when a step's weights sum to more than kMostWeight: sums in
+// fp32 and P's floating-point numbers lose nothing below that, and neither the
+// maximum is taken nor O rescaled in most steps.
 //
 // P is rounded once to the storage type; the row sum l is taken before that.
 // Each output then carries independent errors of half a step per key, which
@@ -41,7 +42,7 @@ constexpr int kBox = 16;       // positions of a box
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kFlagRing = 4;  // steps whose missing-key flags are kept: more than the stages
-constexpr float kSlack = 8.0f;
+constexpr float kMostWeight = 8192.0f;  // of a row in one step; fp16 ends at 65504
 constexpr uint32_t kTmemColumns = 512;
 
 template <int D>
@@ -55,28 +56,16 @@ struct TensorCfg {
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 32 consecutive 32-bit columns of this warp's lanes (one row per thread).
-__device__ __forceinline__ void tmem_load32(uint32_t at, float *v) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(at));
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
+// Consecutive 32-bit columns of this warp's lanes (one row per thread), there
+// when the call returns.
 __device__ __forceinline__ void tmem_load128(uint32_t at, float *v) {
   uint32_t r[128];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];"
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
       : "r"(at));
 #pragma unroll
@@ -85,12 +74,25 @@ __device__ __forceinline__ void tmem_load128(uint32_t at, float *v) {
 __device__ __forceinline__ void tmem_load16(uint32_t at, float *v) {
   uint32_t r[16];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(at));
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_store64(uint32_t at, const uint32_t (&r)[64]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x64.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+      "r"(r[32]), "r"(r[33]), "r"(r[34]), "r"(r[35]), "r"(r[36]), "r"(r[37]), "r"(r[38]), "r"(r[39]),
+      "r"(r[40]), "r"(r[41]), "r"(r[42]), "r"(r[43]), "r"(r[44]), "r"(r[45]), "r"(r[46]), "r"(r[47]),
+      "r"(r[48]), "r"(r[49]), "r"(r[50]), "r"(r[51]), "r"(r[52]), "r"(r[53]), "r"(r[54]), "r"(r[55]),
+      "r"(r[56]), "r"(r[57]), "r"(r[58]), "r"(r[59]), "r"(r[60]), "r"(r[61]), "r"(r[62]), "r"(r[63])
+      : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
@@ -145,6 +147,16 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 0 below the norma
   return y;
 }
 
+// mbar_wait, which reads the clock, only where the barrier is not through yet.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done || mbar_wait(bar, parity);
+}
 // Bits [a, b) of 32.
 __device__ __forceinline__ uint32_t bits_between(int a, int b) {
   a = max(a, 0);
@@ -273,21 +285,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int always = p.sinks < vis.low ? p.sinks : vis.sinks + max(0, min(p.sinks, pos + 1) - vis.low);
     const int from = vis.sinks + max(0, pos - p.window + 1 - vis.low);
     const int to = min(vis.sinks + pos + 1 - vis.low, v1);
+    // Steps that all of the tile's rows see as a whole: those below
+    // `always_all`, and those in [from_all, to_all).
+    const int always_all = min(p.sinks < vis.low ? p.sinks : vis.sinks + max(0, min(p.sinks, p_lo + 1) - vis.low), v1);
+    const int from_all = vis.sinks + max(0, p_hi - p.window + 1 - vis.low);
+    const int to_all = min(vis.sinks + p_lo + 1 - vis.low, v1);
     bool failed = false;
     if (t < tiles) {
       for (int j = 0; j < steps; ++j) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1))) {
+        if (!__all_sync(0xffffffffu, wait(&s_full[t], j & 1))) {
           if (lane == 0) gave_up(j);
           failed = true;
           break;
         }
         fence_after();
-        const int first = v0 + j * kKeys, last = min(first + kKeys, v1) - 1;
-        const int j0 = vis.key(first), j1 = vis.key(last);
-        bool whole = first + kKeys <= v1 && j1 <= p_lo && (j0 > p_hi - p.window || j1 < p.sinks);
+        const int first = v0 + j * kKeys;
+        const bool whole = first + kKeys <= always_all || (first >= from_all && first + kKeys <= to_all);
         if (!whole) {
           const int st = j % S;
-          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / S) & 1))) {
+          if (!__all_sync(0xffffffffu, wait(&v_full[st], (j / S) & 1))) {
             if (lane == 0) gave_up(j);
             failed = true;
             break;
@@ -299,34 +315,58 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (special) marked[t] = 1;
         }
         const bool missing = (bad_any[j % kFlagRing][0] | bad_any[j % kFlagRing][1]) != 0;
-        float x[kKeys];
-        tmem_load128(s_at, x);
-        wait_ld();
-        if (!whole || missing) {
+        const bool masked = !whole || missing;
+        auto load = [&](float (&x)[kKeys]) {
+          tmem_load128(s_at, x);
+          if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int v = first + c * 32;
-            uint32_t bits = bits_between(0 - v, min(always, v1) - v) | bits_between(from - v, to - v);
-            if (missing)
-              for (int i = 0; i < 32; ++i)
-                if (bad_keys[j % kFlagRing][c * 32 + i]) bits &= ~(1u << i);
+            for (int c = 0; c < 4; ++c) {
+              const int v = first + c * 32;
+              uint32_t bits = bits_between(0 - v, min(always, v1) - v) | bits_between(from - v, to - v);
+              if (missing)
+                for (int i = 0; i < 32; ++i)
+                  if (bad_keys[j % kFlagRing][c * 32 + i]) bits &= ~(1u << i);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[c * 32 + i] = (bits >> i) & 1 ? x[c * 32 + i] : -INFINITY;
+              for (int i = 0; i < 32; ++i) x[c * 32 + i] = (bits >> i) & 1 ? x[c * 32 + i] : -INFINITY;
+            }
           }
-        }
-        float mx;
-        {
-          float y[8];
+        };
+        float x[kKeys];
+        uint32_t w[kKeys / 2];  // P, two weights to a register
+        float2 sum[2];
+        auto weigh = [&] {
+          // A masked score (-inf) has weight 0; a row that has seen nothing yet has m = -inf.
+          const float about = m_run == -INFINITY ? 0.0f : -m_run;
+          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = fmaxf(x[i], x[i + 8]);
+          for (int i = 0; i < kKeys / 2; ++i) {
+            const float2 y = __ffma2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(scale, scale),
+                                        make_float2(about, about));
+            const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+            w[i] = pack2(e.x, e.y, E());
+          }
+          return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        };
+        // Weights about the present m; where they are too large, m moves and the
+        // step is weighed again. The first step starts with its maximum.
+        load(x);
+        bool rise = true;
+#pragma unroll 1
+        for (int round = j == 0 ? 1 : 0;; ++round) {
+          if (round != 1) {
+            const float total_weight = weigh();
+            if (round > 1) break;
+            rise = total_weight > kMostWeight || m_run == -INFINITY;
+            if (!__any_sync(0xffffffffu, rise)) break;
+            load(x);
+            continue;
+          }
+          float mx = -INFINITY;
 #pragma unroll
-          for (int i = 16; i < kKeys; i += 16)
-#pragma unroll
-            for (int n = 0; n < 8; ++n) y[n] = fmaxf(y[n], fmaxf(x[i + n], x[i + n + 8]));
-          mx = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))) * scale;
-        }
-        const bool rise = mx > m_run + kSlack;
-        if (__any_sync(0xffffffffu, rise)) {
+          for (int i = 0; i < kKeys; ++i) mx = fmaxf(mx, x[i]);
+          mx *= scale;
+          rise = rise && mx > m_run;
           const float f = rise ? exp2_fast(m_run - mx) : 1.0f;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -339,29 +379,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < D; c += 16) {
               float o[16];
               tmem_load16(o_at + c, o);
-              wait_ld();
-              uint32_t w[16];
+              uint32_t scaled[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * f);
-              tmem_store16(o_at + c, w);
+              for (int i = 0; i < 16; ++i) scaled[i] = __float_as_uint(o[i] * f);
+              tmem_store16(o_at + c, scaled);
             }
           }
         }
-        // A masked score (-inf) has weight 0; a row that has seen nothing yet has m = -inf.
-        const float about = m_run == -INFINITY ? 0.0f : -m_run;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float a = x[c * 32 + 2 * i], b = x[c * 32 + 2 * i + 1];
-            const float2 t = __ffma2_rn(make_float2(a, b), make_float2(scale, scale), make_float2(about, about));
-            const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
-            l_run[i & 1] = __fadd2_rn(l_run[i & 1], e);
-            w[i] = pack2(e.x, e.y, E());
-          }
-          tmem_store16(s_at + c * 16, w);  // over columns of S that have been read
-        }
+        for (int i = 0; i < 2; ++i) l_run[i] = __fadd2_rn(l_run[i], sum[i]);
+        tmem_store64(s_at, w);  // over S, which has been read
         wait_st();
         fence_before();
         __syncwarp();
@@ -419,7 +446,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < D / 2; c += 16) {
               float x[16];
               tmem_load16(o_at + part * (D / 2) + c, x);
-              wait_ld();
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<float4 *>(own_rows + swizzled(r, c / 4 + i)) =
@@ -432,7 +458,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < D; c += 16) {
             float x[16];
             tmem_load16(o_at + c, x);
-            wait_ld();
 #pragma unroll
             for (int i = 0; i < 2; ++i)
               *reinterpret_cast<uint4 *>(own_rows + swizzled(r, c / 8 + i)) =
@@ -464,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
       next = find(j + 1);
       uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
-      if (j >= S && !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / S) - 1) & 1))) {
+      if (j >= S && !__all_sync(0xffffffffu, wait(&empty[st], ((j / S) - 1) & 1))) {
         if (lane == 0) gave_up(j);
         break;
       }
@@ -534,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         next[i] = find(job + kLoadWarps, i);
       }
       uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
-      if (j >= S && !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((j / S) - 1) & 1))) {
+      if (j >= S && !__all_sync(0xffffffffu, wait(&empty[st], ((j / S) - 1) & 1))) {
         if (lane == 0) gave_up(j);
         break;
       }
@@ -575,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       commit(&s_full[t]);
     };
-    ok = ok && mbar_wait(&k_full[0], 0);
+    ok = ok && wait(&k_full[0], 0);
     fence_after();
     if (ok) {
       for (int t = 0; t < tiles; ++t) scores(t, 0);
@@ -583,10 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int j = 0; j < steps && ok; ++j) {
       const int st = j % S;
-      ok = mbar_wait(&v_full[st], (j / S) & 1);
-      if (j + 1 < steps) ok = ok && mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1);
+      ok = wait(&v_full[st], (j / S) & 1);
+      if (j + 1 < steps) ok = ok && wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1);
       for (int t = 0; t < tiles && ok; ++t) {
-        ok = mbar_wait(&p_full[t], j & 1);
+        ok = wait(&p_full[t], j & 1);
         if (!ok) break;
         fence_after();
         const uint32_t v = smem_u32(sV + st * C::kTile);
