@@ -732,6 +732,7 @@ cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t str
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 0;
+  pdl = true;  // its launch overlaps the splits' end, which it waits for
   add_pdl();
   return cudaLaunchKernelEx(&cfg, window_join_kernel<E, D>, p, plan.outer);
 }

@@ -186,6 +186,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int marked[2];  // the tile met an infinity or NaN beside masked pairs
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (BOXES && tid < 2)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tid ? &v_map : &k_map)) : "memory");
   pdl_wait();
   const int s = blockIdx.z, h = blockIdx.y, split = (gridDim.x - 1 - blockIdx.x) % splits;
   const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
@@ -214,6 +216,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           make_float2(-INFINITY, 0.0f);
     return;
   }
+
+  auto find_box = [&](int j) {  // lane i < 8: group i of step j
+    const int v = v0 + j * kKeys + lane * kBox;
+    return lane < kKeys / kBox && j < steps && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
+  };
+  KeyPlace first_box{0, -1, 0};
+  if (BOXES && warp >= kSoftmaxWarps && warp < kMmaWarp) first_box = find_box(0);  // on its way over the barrier
 
   if (warp == kMmaWarp) {
     if (lane == 0) {
@@ -475,11 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- loads by boxes: a warp for K, a warp for V, lane i < 8 takes group i of a step ----
     const int load = warp - kSoftmaxWarps;
     const bool value = load == 1;
-    auto find = [&](int j) {
-      const int v = v0 + j * kKeys + lane * kBox;
-      return lane < kKeys / kBox && j < steps && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
-    };
-    KeyPlace next = find(0);
+    KeyPlace next = first_box;
     uint32_t edges = 0;  // steps whose V rows were cleaned: the phase of v_landed
     for (int j = 0; j < steps && load < 2; ++j) {
       const int st = j % S, first = v0 + j * kKeys;
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const long long row = here ? pool_row(p, next, h, s) : -1;
       const unsigned bad = __ballot_sync(0xffffffffu, here && row < 0);
       const int boxes = __popc(__ballot_sync(0xffffffffu, row >= 0));
-      next = find(j + 1);
+      next = find_box(j + 1);
       uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
       if (j >= S && !__all_sync(0xffffffffu, wait(&empty[st], ((j / S) - 1) & 1))) {
         if (lane == 0) gave_up(j);
