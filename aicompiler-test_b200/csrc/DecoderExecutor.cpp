@@ -9,10 +9,13 @@
 #include <stdexcept>
 
 #include "attention.cuh"
+#include "cache_ops.cuh"
 #include "gemm.cuh"
 #include "gemv.cuh"
 #include "half_convert.hpp"
+#include "logprobs.cuh"
 #include "misc.cuh"
+#include "window_attention.cuh"
 
 namespace tensor::runtime {
 
@@ -710,17 +713,142 @@ std::string DecoderExecutor::restorePages(int slot, const KVPageSnapshot &snap) 
   return {};
 }
 
-std::string DecoderExecutor::ensureSpill(std::size_t bytes, int npages) {
-  if (!poolPtrs_) {
-    std::vector<void *> ptrs;
-    for (const auto &L : layers_) {
-      ptrs.push_back(L.kPool->data());
-      ptrs.push_back(L.vPool->data());
+std::string DecoderExecutor::ensurePoolPointers() {
+  if (poolPtrs_) return {};
+  std::vector<void *> ptrs;
+  for (const auto &L : layers_) {
+    ptrs.push_back(L.kPool->data());
+    ptrs.push_back(L.vPool->data());
+  }
+  auto r = rt_.createBuffer(ptrs.size() * 2, nullptr, ElementType::Int32);  // 8-byte pointers as int32 pairs
+  if (!r.buffer) return r.errorMessage;
+  TMC_TRY(cudaMemcpy(r.buffer->data(), ptrs.data(), ptrs.size() * sizeof(void *), cudaMemcpyHostToDevice));
+  poolPtrs_ = r.buffer;
+  return {};
+}
+
+// Every user of the lists synchronises before it returns.
+std::string DecoderExecutor::ensurePageLists(std::size_t count) {
+  if (pageLists_ && pageLists_->elementCount() >= count) return {};
+  auto r = rt_.createBuffer(std::max<std::size_t>(count, 64), nullptr, ElementType::Int32);
+  if (!r.buffer) return r.errorMessage;
+  pageLists_ = r.buffer;
+  return {};
+}
+
+std::string DecoderExecutor::copyPages(const std::vector<KVPageCopy> &copies) {
+  if (copies.empty()) return {};
+  if (auto e = ensurePoolPointers(); !e.empty()) return e;
+  const std::size_t n = copies.size();
+  if (auto e = ensurePageLists(2 * n); !e.empty()) return e;
+  std::vector<std::int32_t> lists(2 * n);
+  for (std::size_t i = 0; i < n; ++i) {
+    lists[i] = copies[i].from;
+    lists[n + i] = copies[i].to;
+  }
+  auto *device = static_cast<std::int32_t *>(pageLists_->data());
+  const std::size_t pageBytes = (std::size_t)hkvL_ * pageSize_ * cfg_.headDim * 2;
+  TMC_TRY(cudaMemcpyAsync(device, lists.data(), lists.size() * 4, cudaMemcpyHostToDevice, rt_.stream()));
+  TMC_TRY(tmc::launch_kv_copy_pages(static_cast<void *const *>(poolPtrs_->data()), 2 * cfg_.layers, poolPages_, pageBytes,
+                                    device, device + n, (int)n, rt_.deviceStatus(), rt_.stream()));
+  TMC_TRY(cudaStreamSynchronize(rt_.stream()));  // `lists` is read until then
+  return {};
+}
+
+std::string DecoderExecutor::prepareAppend(int slot) {
+  std::vector<KVPageCopy> copies;
+  auto e = slots_[slot]->unshareTail(&copies);
+  return e.empty() ? copyPages(copies) : e;
+}
+
+std::string DecoderExecutor::forkSlot(int slot, const std::int32_t *slots, int count) {
+  if (slot < 0 || slot >= cfg_.maxSlots || slots == nullptr) return "fork: slot out of range.";
+  if (count < 1) return "fork: slot count must be positive.";
+  if ((std::size_t)hkvL_ * pageSize_ * cfg_.headDim % 8 != 0) return "fork: KV pages must be multiples of 16 bytes.";
+  for (int i = 0; i < count; ++i) {
+    if (slots[i] < 0 || slots[i] >= cfg_.maxSlots) return "fork: slot out of range.";
+    if (slots[i] == slot) return "fork: a slot cannot be its own fork.";
+    for (int q = 0; q < i; ++q)
+      if (slots[q] == slots[i]) return "fork: slots must be distinct.";
+  }
+  std::vector<KVPageCopy> copies;
+  std::string e;
+  int made = 0;
+  for (; made < count && e.empty(); ++made) e = slots_[slots[made]]->fork(*slots_[slot], &copies);
+  if (!e.empty()) --made;
+  if (e.empty()) e = copyPages(copies);
+  if (!e.empty())
+    for (int i = 0; i < made; ++i) (void)slots_[slots[i]]->reset();
+  return e;
+}
+
+std::string DecoderExecutor::compactSlot(int slot, const std::int32_t *keep, int count) {
+  if (slot < 0 || slot >= cfg_.maxSlots || keep == nullptr) return "compact: slot out of range.";
+  auto &st = *slots_[slot];
+  const std::size_t length = st.currentLength(), P = pageSize_;
+  if (count < 1 || (std::size_t)count > length) return "compact: kept positions must be in [1, length].";
+  for (int i = 0; i < count; ++i)
+    if (keep[i] < 0 || (std::size_t)keep[i] >= length || (i > 0 && keep[i] <= keep[i - 1]))
+      return "compact: kept positions must ascend within the committed length.";
+  if (cfg_.headDim % 8 != 0) return "compact: head dimension must be a multiple of 8.";
+  std::size_t same = 0;  // rows that stay where they are
+  while (same < (std::size_t)count && keep[same] == (std::int32_t)same) ++same;
+  if (same == (std::size_t)count) return rollbackLength(slot, count);
+  const std::size_t lead = same / P, pages = ((std::size_t)count + P - 1) / P - lead, first = lead * P;
+  std::vector<std::int32_t> fresh;
+  auto giveBack = [&] {
+    for (auto page : fresh) pool_->releasePage(page);
+  };
+  for (std::size_t i = 0; i < pages; ++i) {
+    const auto page = pool_->allocatePage();
+    if (page < 0) {
+      giveBack();
+      return "Paged KV cache physical page pool is exhausted.";
     }
-    auto r = rt_.createBuffer(ptrs.size() * 2, nullptr, ElementType::Int32);  // 8-byte pointers as int32 pairs
-    if (!r.buffer) return r.errorMessage;
-    poolPtrs_ = r.buffer;
-    TMC_TRY(cudaMemcpy(poolPtrs_->data(), ptrs.data(), ptrs.size() * sizeof(void *), cudaMemcpyHostToDevice));
+    fresh.push_back(page);
+  }
+  // Device lists: the sequence's pages, the new ones (by new position), the kept positions.
+  const auto old = st.pageTable();
+  std::vector<std::int32_t> lists(old);
+  lists.insert(lists.end(), old.begin(), old.begin() + (std::ptrdiff_t)lead);
+  lists.insert(lists.end(), fresh.begin(), fresh.end());
+  lists.insert(lists.end(), keep + first, keep + count);
+  std::string e = ensurePoolPointers();
+  if (e.empty()) e = ensurePageLists(lists.size());
+  if (e.empty()) {
+    auto *device = static_cast<std::int32_t *>(pageLists_->data());
+    tmc::CompactParams c{};
+    c.pools = static_cast<void *const *>(poolPtrs_->data());
+    c.layers = cfg_.layers;
+    c.pool_pages = poolPages_;
+    c.hkv = hkvL_;
+    c.d = cfg_.headDim;
+    c.page_size = pageSize_;
+    c.src_pages = device;
+    c.src_count = (int)old.size();
+    c.dst_pages = device + old.size();
+    c.dst_count = (int)(lead + pages);
+    c.keep = device + old.size() + lead + pages;
+    c.count = count - (int)first;
+    c.first = (int)first;
+    c.cos = fp(ropeCos_);
+    c.sin = fp(ropeSin_);
+    c.rope_rows = cfg_.capacity;
+    c.status = rt_.deviceStatus();
+    cudaError_t ce = cudaMemcpyAsync(device, lists.data(), lists.size() * 4, cudaMemcpyHostToDevice, rt_.stream());
+    if (ce == cudaSuccess) ce = tmc::launch_kv_compact(c, false, rt_.stream());
+    if (ce != cudaSuccess) e = cudaText("compact", ce);
+    const std::string sync = rt_.synchronize();
+    if (e.empty()) e = sync;
+  }
+  if (e.empty()) e = st.replaceTail(lead, fresh, count);
+  if (!e.empty()) giveBack();
+  return e;
+}
+
+std::string DecoderExecutor::ensureSpill(std::size_t bytes, int npages) {
+  if (auto e = ensurePoolPointers(); !e.empty()) return e;
+  if (!spillPages_) {
     auto q = rt_.createBuffer((size_t)maxPagesPerSeq_, nullptr, ElementType::Int32);
     if (!q.buffer) return q.errorMessage;
     spillPages_ = q.buffer;
@@ -790,7 +918,10 @@ std::string DecoderExecutor::restoreKV(int slot, std::size_t length,
 int DecoderExecutor::kernelsPerStep(int rows) const {
   const bool tp = cfg_.tpSize > 1;
   // Batched steps add a prologue kernel before the QKV, gate/up and LM-head projections.
-  const int perLayer = rows > kGemvMaxRows ? 7 : 5;
+  int perLayer = rows > kGemvMaxRows ? 7 : 5;
+  if (window_ > 0)
+    perLayer += tmc::window_attention_launches(rows, 1, hqL_, hkvL_, cfg_.headDim, window_, sinks_, cfg_.capacity,
+                                               numSms_) - 1;
   const int head = rows > kGemvMaxRows ? 2 : 1;
   return cfg_.layers * perLayer + head + (tp && !peersAttached_ ? 1 : 0);  // + argmax finalize after the collective
 }
@@ -802,7 +933,10 @@ double DecoderExecutor::stepAlgorithmicBytes(int rows, const std::vector<int> &c
   w *= cfg_.layers;
   w += (double)vL_ * H + H;  // LM head + final norm
   double bytes = 2.0 * w + 2.0 * rows * H;  // weights + embedding rows
-  for (int c : ctx) bytes += 2.0 * 2.0 * hkvL_ * D * c * cfg_.layers;  // K and V reads
+  for (int c : ctx) {  // K and V reads
+    const double seen = window_ > 0 ? std::min<double>(c, (double)window_ + sinks_) : c;
+    bytes += 2.0 * 2.0 * hkvL_ * D * seen * cfg_.layers;
+  }
   bytes += 2.0 * 2.0 * hkvL_ * D * rows * cfg_.layers;                // K and V appends
   return bytes;
 }
@@ -1040,7 +1174,38 @@ std::string DecoderExecutor::enqueueKernel(int kind, int l, int R, bool feed, bo
     case kKernelQKV:
       return launchProjection(projection(kind, l, R, feed), "qkv projection");
     case kKernelAttention: {
-
+      if (window_ > 0) {
+        tmc::WindowAttentionParams w{};
+        w.q = hp(q_);
+        w.q_stride = w.out_stride = (long long)hqL_ * D;
+        w.out = hp(ctx_);
+        w.k_pool = hp(L.kPool);
+        w.v_pool = hp(L.vPool);
+        w.block_table = static_cast<const int *>(blockTable_->data());
+        w.table_stride = maxPagesPerSeq_;
+        w.table_rows = tableRows;
+        w.first_positions = positions;
+        const int *starts = static_cast<const int *>(rowStarts_->data());
+        w.row_starts = distinct ? starts : starts + cfg_.maxRows + 1 + 2 * R;
+        w.sequences = distinct ? R : 1;
+        w.rows = R;
+        w.max_rows = distinct ? 1 : R;
+        w.hq = hqL_;
+        w.hkv = hkvL_;
+        w.d = D;
+        w.page_size = pageSize_;
+        w.pool_pages = poolPages_;
+        w.capacity = cfg_.capacity;
+        w.window = window_;
+        w.sinks = sinks_;
+        w.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)));
+        w.workspace = windowWorkspace_ ? windowWorkspace_->data() : nullptr;
+        w.workspace_bytes = windowWorkspace_ ? windowWorkspace_->byteCount() : 0;
+        w.status = status;
+        if ((e = tmc::launch_window_attention(w, false, numSms_, s, pdl)) != cudaSuccess)
+          return cudaText("window attention", e);
+        return {};
+      }
       tmc::AttentionParams a{};
       a.q = hp(q_);
       a.q_stride = (long long)hqL_ * D;
@@ -1323,7 +1488,8 @@ std::string DecoderExecutor::decode(const std::int32_t *slots, const std::int32_
     auto &st = *slots_[slots[staged]];
     positions[staged] = static_cast<std::int32_t>(st.currentLength());
     tableRows[staged] = slots[staged];
-    err = st.stageLength(st.currentLength() + 1);
+    err = prepareAppend(slots[staged]);
+    if (err.empty()) err = st.stageLength(st.currentLength() + 1);
     if (!err.empty()) break;
   }
   auto unwind = [&](int n) {
@@ -1339,6 +1505,7 @@ std::string DecoderExecutor::decode(const std::int32_t *slots, const std::int32_
     cudaEventCreate(&e1);
   }
   const auto c0 = std::chrono::steady_clock::now();
+  logitRows_ = 0;
   err = uploadStepInputs(rows, tokens, positions.data(), tableRows.data());
   if (timing) cudaEventRecord(e0, rt_.stream());
   if (err.empty()) err = launchStep(rows, false, true);
@@ -1368,25 +1535,142 @@ std::string DecoderExecutor::decode(const std::int32_t *slots, const std::int32_
     st.commitLength(st.currentLength() + 1);
     if (nextTokens) nextTokens[r] = pinnedIO_[3 * cfg_.maxRows + r];
   }
+  logitRows_ = rows;
   return {};
 }
 
 std::string DecoderExecutor::prefill(int slot, const std::int32_t *tokens, int count, float *logits,
                                      std::int32_t *nextToken, StepTiming *timing) {
+  return runPrefill(slot, tokens, count, logits, nextToken, timing, nullptr);
+}
+
+std::string DecoderExecutor::score(int slot, const std::int32_t *tokens, int count, const TokenScores &out,
+                                   std::int32_t *nextToken) {
+  if (auto e = ensureScores(); !e.empty()) return e;
+  return runPrefill(slot, tokens, count, nullptr, nextToken, nullptr, &out);
+}
+
+std::string DecoderExecutor::ensureScores() {
+  if (cfg_.tpSize > 1) return "token scores need the whole vocabulary on one rank (tensor parallelism splits it).";
+  if (scoreTargets_) return {};
+  const std::size_t M = cfg_.maxRows, top = tmc::kLogprobsMaxTop;
+  auto f = rt_.createBuffer(M * (2 + top), nullptr, ElementType::Float32);
+  if (!f.buffer) return f.errorMessage;
+  auto i = rt_.createBuffer(M * (1 + top), nullptr, ElementType::Int32);
+  if (!i.buffer) return i.errorMessage;
+  auto t = rt_.createBuffer(M, nullptr, ElementType::Int32);
+  if (!t.buffer) return t.errorMessage;
+  scoreFloats_ = f.buffer;
+  scoreInts_ = i.buffer;
+  scoreTargets_ = t.buffer;
+  return {};
+}
+
+std::string DecoderExecutor::enqueueScores(const std::int32_t *targets, int rows, const TokenScores &out,
+                                           std::size_t at) {
+  cudaStream_t s = rt_.stream();
+  const std::size_t M = cfg_.maxRows;
+  auto *floats = fp(scoreFloats_);
+  auto *ints = static_cast<std::int32_t *>(scoreInts_->data());
+  tmc::LogprobsParams p{};
+  p.logits = fp(logits_);
+  p.row_stride = vL_;
+  p.targets = static_cast<const int *>((targets ? scoreTargets_ : nextTokens_)->data());
+  p.rows = rows;
+  p.vocab = vL_;
+  p.top = out.top;
+  p.logprobs = floats;
+  p.entropy = floats + M;
+  p.top_logprobs = floats + 2 * M;
+  p.ranks = ints;
+  p.top_ids = ints + M;
+  p.status = rt_.deviceStatus();
+  if (targets)
+    TMC_TRY(cudaMemcpyAsync(scoreTargets_->data(), targets, sizeof(std::int32_t) * rows, cudaMemcpyHostToDevice, s));
+  TMC_TRY(tmc::launch_token_logprobs(p, tmc::kLogitsF32, numSms_, s));
+  const std::size_t n = rows, k = out.top;
+  auto fetch = [&](void *host, const void *device, std::size_t count) {
+    return host && count ? cudaMemcpyAsync(host, device, count * 4, cudaMemcpyDeviceToHost, s) : cudaSuccess;
+  };
+  TMC_TRY(fetch(out.logprobs ? out.logprobs + at : nullptr, p.logprobs, n));
+  TMC_TRY(fetch(out.entropy ? out.entropy + at : nullptr, p.entropy, n));
+  TMC_TRY(fetch(out.ranks ? out.ranks + at : nullptr, p.ranks, n));
+  TMC_TRY(fetch(out.topIds ? out.topIds + at * k : nullptr, p.top_ids, n * k));
+  TMC_TRY(fetch(out.topLogprobs ? out.topLogprobs + at * k : nullptr, p.top_logprobs, n * k));
+  return {};
+}
+
+std::string DecoderExecutor::tokenScores(const std::int32_t *targets, int rows, const TokenScores &out) {
+  if (rows < 1 || rows > logitRows_) return "token scores: rows must be in [1, rows of the last step].";
+  for (int r = 0; targets && r < rows; ++r)
+    if (targets[r] < -1 || targets[r] >= cfg_.vocab) return "token scores: target out of vocabulary range.";
+  auto e = ensureScores();
+  if (e.empty()) e = enqueueScores(targets, rows, out, 0);
+  const std::string sync = rt_.synchronize();
+  return e.empty() ? sync : e;
+}
+
+std::string DecoderExecutor::setWindow(int window, int sinks) {
+  if (window < 0 || sinks < 0) return "window and sinks must not be negative.";
+  const int D = cfg_.headDim;
+  if (window > 0 && D != 16 && D != 32 && D != 64 && D != 128)
+    return "window attention needs a head dimension of 16, 32, 64 or 128.";
+  TMC_TRY(cudaStreamSynchronize(rt_.stream()));
+  const int M = cfg_.maxRows;
+  if (window > 0 && !rowStarts_) {
+    std::vector<std::int32_t> starts((std::size_t)M + 1 + 2 * ((std::size_t)M + 1), 0);
+    for (int i = 0; i <= M; ++i) {
+      starts[i] = i;
+      starts[M + 1 + 2 * i + 1] = i;
+    }
+    auto r = rt_.createBuffer(starts.size(), nullptr, ElementType::Int32);
+    if (!r.buffer) return r.errorMessage;
+    TMC_TRY(cudaMemcpy(r.buffer->data(), starts.data(), starts.size() * 4, cudaMemcpyHostToDevice));
+    rowStarts_ = r.buffer;
+  }
+  if (window > 0) {
+    std::size_t bytes = 0;
+    for (int r = 1; r <= M; ++r) {
+      bytes = std::max(bytes, tmc::window_attention_workspace_bytes(r, 1, hqL_, hkvL_, cfg_.headDim,
+                                                                    std::min(window, cfg_.capacity), sinks, numSms_));
+      bytes = std::max(bytes, tmc::window_attention_workspace_bytes(1, r, hqL_, hkvL_, cfg_.headDim,
+                                                                    std::min(window, cfg_.capacity), sinks, numSms_));
+    }
+    if (bytes > 0 && (!windowWorkspace_ || windowWorkspace_->byteCount() < bytes)) {
+      auto r = rt_.createBuffer(bytes / 4 + 1, nullptr, ElementType::Float32);
+      if (!r.buffer) return r.errorMessage;
+      windowWorkspace_ = r.buffer;
+    }
+  }
+  window_ = window;
+  sinks_ = window > 0 ? sinks : 0;
+  dropGraphs();
+  return {};
+}
+
+std::string DecoderExecutor::runPrefill(int slot, const std::int32_t *tokens, int count, float *logits,
+                                        std::int32_t *nextToken, StepTiming *timing, const TokenScores *scores) {
   if (slot < 0 || slot >= cfg_.maxSlots) return "prefill: slot out of range.";
   if (count < 1) return "prefill: token count must be positive.";
   for (int i = 0; i < count; ++i)
     if (tokens[i] < 0 || tokens[i] >= cfg_.vocab) return "prefill: token id out of vocabulary range.";
   auto &st = *slots_[slot];
   const size_t start = st.currentLength();
-  auto err = st.stageLength(start + count);
+  auto err = prepareAppend(slot);
+  if (err.empty()) err = st.stageLength(start + count);
   if (!err.empty()) return err;
+  std::vector<std::int32_t> targets;  // of every position: the token behind it
+  if (scores) {
+    targets.assign(tokens + 1, tokens + count);
+    targets.push_back(-1);
+  }
   // Chunks of maxRows rows (the reference's prefillChunked,
   // DecoderLLMExecutor.cpp:982-1034), queued back to back: each chunk's inputs
   // come from its own pinned staging block, so the host never waits between
   // chunks; one synchronisation at the end (per chunk only when logits are
   // copied to pageable host memory).
   const int M = cfg_.maxRows;
+  logitRows_ = 0;
   std::vector<std::int32_t> pos(M), trow(M, slot);
   double gpuUs = 0.0;
   const auto c0 = std::chrono::steady_clock::now();
@@ -1407,13 +1691,14 @@ std::string DecoderExecutor::prefill(int slot, const std::int32_t *tokens, int c
     err = uploadStepInputs(R, tokens + done, pos.data(), trow.data(), 1, prefillStage_ + (std::size_t)chunk * 3 * M);
     // Only the last chunk's LM head is read unless logits are asked for (the
     // peer exchange's step epoch advances in the head, so it always runs then).
-    const bool head = logits != nullptr || done + R == count || (cfg_.tpSize > 1 && peersAttached_);
+    const bool head = logits != nullptr || scores != nullptr || done + R == count || (cfg_.tpSize > 1 && peersAttached_);
     if (err.empty()) err = launchStep(R, false, R == 1, head);
     if (err.empty() && logits) {
       cudaError_t ce = cudaMemcpyAsync(logits + (size_t)done * vL_, logits_->data(), sizeof(float) * R * vL_,
                                        cudaMemcpyDeviceToHost, rt_.stream());
       if (ce != cudaSuccess) err = cudaText("prefill logits readback", ce);
     }
+    if (err.empty() && scores) err = enqueueScores(targets.data() + done, R, *scores, (std::size_t)done);
     if (err.empty() && done + R == count) {
       cudaError_t ce = cudaMemcpyAsync(pinnedIO_ + 3 * M, nextTokens_->data(), sizeof(std::int32_t) * R,
                                        cudaMemcpyDeviceToHost, rt_.stream());
@@ -1441,6 +1726,7 @@ std::string DecoderExecutor::prefill(int slot, const std::int32_t *tokens, int c
     return err;
   }
   st.commitLength(start + count);
+  logitRows_ = last;
   return {};
 }
 
@@ -1462,7 +1748,8 @@ std::string DecoderExecutor::generate(const std::int32_t *slots, const std::int3
     auto &st = *slots_[slots[staged]];
     positions[staged] = static_cast<std::int32_t>(st.currentLength());
     tableRows[staged] = slots[staged];
-    err = st.stageLength(st.currentLength() + steps);
+    err = prepareAppend(slots[staged]);
+    if (err.empty()) err = st.stageLength(st.currentLength() + steps);
     if (!err.empty()) break;
   }
   auto unwind = [&](int n) {
@@ -1476,6 +1763,7 @@ std::string DecoderExecutor::generate(const std::int32_t *slots, const std::int3
   cudaEventCreate(&e0);
   cudaEventCreate(&e1);
   const auto c0 = std::chrono::steady_clock::now();
+  logitRows_ = 0;
   err = uploadStepInputs(rows, tokens, positions.data(), tableRows.data(), steps);
   if (err.empty()) {
     cudaError_t ce = cudaMemsetAsync(historyCounter_->data(), 0, 4, rt_.stream());
@@ -1533,6 +1821,7 @@ std::string DecoderExecutor::generate(const std::int32_t *slots, const std::int3
     auto &st = *slots_[slots[r]];
     st.commitLength(st.currentLength() + steps);
   }
+  logitRows_ = rows;
   return {};
 }
 

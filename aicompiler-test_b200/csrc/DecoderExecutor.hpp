@@ -171,6 +171,32 @@ class DecoderExecutor {
   std::string commitLength(int slot, std::size_t length);
   std::string rollbackLength(int slot, std::size_t length);
   std::string releaseSlot(int slot);
+  // ---- forks, compaction, scores, windows (no reference counterpart) ----
+  // Every slot of `slots` (empty ones) becomes a copy of `slot`: the full pages
+  // are shared, the partly filled one is copied in every layer (one kernel).
+  std::string forkSlot(int slot, const std::int32_t *slots, int count);
+  // Keep only the `count` committed positions keep[] (ascending) of a sequence:
+  // kept row i becomes position i, keys turned back by the distance moved
+  // (one kernel over all layers). Leading pages that keep all of their rows stay.
+  std::string compactSlot(int slot, const std::int32_t *keep, int count);
+  // Host results of token scores, [rows] and [rows, top]; unwanted ones null.
+  struct TokenScores {
+    float *logprobs = nullptr;
+    float *entropy = nullptr;
+    std::int32_t *ranks = nullptr;
+    int top = 0;
+    std::int32_t *topIds = nullptr;
+    float *topLogprobs = nullptr;
+  };
+  // Scores of targets[r] (null: of the greedy tokens) under row r of the last
+  // step's logits (a prefill's last chunk).
+  std::string tokenScores(const std::int32_t *targets, int rows, const TokenScores &out);
+  // prefill that scores every position's next token tokens[i + 1] on the device
+  // (the last position has none: log probability 0, rank -1).
+  std::string score(int slot, const std::int32_t *tokens, int count, const TokenScores &out, std::int32_t *nextToken);
+  // Attend only to the newest `window` positions (the query's own included) and
+  // to the first `sinks`; window 0: to all, by the kernels without a window.
+  std::string setWindow(int window, int sinks);
   std::vector<std::int32_t> blockTable(int slot) const;
   // [localKVHeads, length, headDim] logical values (reference readKeyPrefix).
   std::string readKV(int layer, int slot, std::vector<float> *key, std::vector<float> *value) const;
@@ -194,6 +220,16 @@ class DecoderExecutor {
 
  private:
   std::string ensureSpill(std::size_t bytes, int npages);
+  std::string ensurePoolPointers();
+  std::string ensurePageLists(std::size_t count);
+  std::string copyPages(const std::vector<KVPageCopy> &copies);
+  // A slot's next position falls into a page of its own.
+  std::string prepareAppend(int slot);
+  std::string ensureScores();
+  // Scores of `rows` rows of logits_ into host memory at row `at`, enqueued.
+  std::string enqueueScores(const std::int32_t *targets, int rows, const TokenScores &out, std::size_t at);
+  std::string runPrefill(int slot, const std::int32_t *tokens, int count, float *logits, std::int32_t *nextToken,
+                         StepTiming *timing, const TokenScores *scores);
 
  public:
 
@@ -268,7 +304,15 @@ class DecoderExecutor {
   std::size_t prefillChunks_ = 0;
   // Page spill / restore: device array of the 2 * layers pool pointers, page-id
   // list, packed device staging and pinned host staging (grown on demand).
-  cuda::BufferHandle poolPtrs_, spillPages_;
+  cuda::BufferHandle poolPtrs_, spillPages_, pageLists_;
+  // Token scores: targets, then per row log probability, entropy, rank, and the
+  // top lists (allocated on first use); rows of logits that the last step left.
+  cuda::BufferHandle scoreTargets_, scoreFloats_, scoreInts_;
+  int logitRows_ = 0;
+  // Window attention: 0 = off; row ranges of a step (0 .. maxRows for one row
+  // per sequence, then pairs {0, R} for R rows of one sequence), workspace.
+  int window_ = 0, sinks_ = 0;
+  cuda::BufferHandle rowStarts_, windowWorkspace_;
   void *spillDevice_ = nullptr, *spillHost_ = nullptr;
   std::size_t spillBytes_ = 0;
   int historyCapacity_ = 0;

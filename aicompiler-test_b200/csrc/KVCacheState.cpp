@@ -8,7 +8,7 @@
 namespace tensor::runtime {
 
 KVPagePool::KVPagePool(std::size_t pageSize, std::size_t physicalPageCount)
-    : pageSize_(pageSize), allocated_(physicalPageCount, false) {
+    : pageSize_(pageSize), owners_(physicalPageCount, 0) {
   if (pageSize == 0 || physicalPageCount == 0 ||
       physicalPageCount > static_cast<std::size_t>(std::numeric_limits<std::int32_t>::max()))
     throw std::invalid_argument("KV page pool dimensions are invalid.");
@@ -20,8 +20,16 @@ KVPagePool::KVPagePool(std::size_t pageSize, std::size_t physicalPageCount)
 }
 
 bool KVPagePool::isAllocated(std::int32_t page) const noexcept {
-  return page >= 0 && static_cast<std::size_t>(page) < allocated_.size() &&
-         allocated_[static_cast<std::size_t>(page)];
+  return owners(page) > 0;
+}
+
+std::size_t KVPagePool::owners(std::int32_t page) const noexcept {
+  return page >= 0 && static_cast<std::size_t>(page) < owners_.size() ? owners_[static_cast<std::size_t>(page)] : 0;
+}
+
+void KVPagePool::retainPage(std::int32_t page) {
+  if (!isAllocated(page)) throw std::invalid_argument("Paged KV attempted to share an invalid page.");
+  ++owners_[static_cast<std::size_t>(page)];
 }
 
 std::int32_t KVPagePool::allocatePage() {
@@ -32,7 +40,7 @@ std::int32_t KVPagePool::allocatePage() {
   if (freePages_.empty()) return -1;
   const auto page = freePages_.back();
   freePages_.pop_back();
-  allocated_[static_cast<std::size_t>(page)] = true;
+  owners_[static_cast<std::size_t>(page)] = 1;
   ++allocationCount_;
   peakUsedPages_ = std::max(peakUsedPages_, usedPages());
   return page;
@@ -40,7 +48,7 @@ std::int32_t KVPagePool::allocatePage() {
 
 void KVPagePool::releasePage(std::int32_t page) {
   if (!isAllocated(page)) throw std::invalid_argument("Paged KV attempted to release an invalid page.");
-  allocated_[static_cast<std::size_t>(page)] = false;
+  if (--owners_[static_cast<std::size_t>(page)] > 0) return;
   freePages_.push_back(page);
   ++releaseCount_;
 }
@@ -143,6 +151,77 @@ std::string KVCacheState::rollbackLength(std::size_t length) {
 void KVCacheState::commitLength(std::size_t length) {
   if (length == 0 || length > capacity_) throw std::invalid_argument("Cannot commit an invalid KV cache length.");
   currentLength_ = length;
+}
+
+std::string KVCacheState::fork(const KVCacheState &source, std::vector<KVPageCopy> *copies) {
+  if (currentLength_ != 0 || allocatedPageCount() != 0) return "A fork needs an empty sequence.";
+  const auto length = source.currentLength_, size = pool_->pageSize();
+  if (pool_ != source.pool_ || length == 0 || length > capacity_) return "A fork needs a sequence of the same pool to fork from.";
+  const auto full = length / size, pages = (length + size - 1) / size;
+  std::int32_t tail = -1;
+  if (pages > full) {
+    tail = pool_->allocatePage();
+    if (tail < 0) return "Paged KV cache physical page pool is exhausted.";
+  }
+  for (std::size_t i = 0; i < full; ++i) {
+    pool_->retainPage(source.logicalToPhysical_[i]);
+    logicalToPhysical_[i] = source.logicalToPhysical_[i];
+  }
+  if (tail >= 0) logicalToPhysical_[full] = tail;
+  if (sink_) {
+    const auto error = sink_(slot_, logicalToPhysical_);
+    if (!error.empty()) {
+      (void)resizePageAllocation(0);
+      (void)sink_(slot_, logicalToPhysical_);
+      return error;
+    }
+  }
+  if (tail >= 0) copies->push_back({source.logicalToPhysical_[full], tail});
+  currentLength_ = length;
+  return {};
+}
+
+std::string KVCacheState::unshareTail(std::vector<KVPageCopy> *copies) {
+  const auto logical = currentLength_ / pool_->pageSize();
+  if (logical >= logicalToPhysical_.size()) return {};
+  const auto shared = logicalToPhysical_[logical];
+  if (pool_->owners(shared) < 2) return {};
+  const auto page = pool_->allocatePage();
+  if (page < 0) return "Paged KV cache physical page pool is exhausted.";
+  logicalToPhysical_[logical] = page;
+  if (sink_) {
+    const auto error = sink_(slot_, logicalToPhysical_);
+    if (!error.empty()) {
+      logicalToPhysical_[logical] = shared;
+      pool_->releasePage(page);
+      (void)sink_(slot_, logicalToPhysical_);
+      return error;
+    }
+  }
+  pool_->releasePage(shared);
+  copies->push_back({shared, page});
+  return {};
+}
+
+std::string KVCacheState::replaceTail(std::size_t lead, const std::vector<std::int32_t> &pages, std::size_t length) {
+  const auto allocated = allocatedPageCount();
+  if (length == 0 || length > capacity_ || lead > allocated || lead + pages.size() > logicalToPhysical_.size() ||
+      length > (lead + pages.size()) * pool_->pageSize())
+    return "KV cache pages do not hold the new length.";
+  auto row = logicalToPhysical_;
+  for (std::size_t i = lead; i < row.size(); ++i) row[i] = i < lead + pages.size() ? pages[i - lead] : -1;
+  std::swap(row, logicalToPhysical_);
+  if (sink_) {
+    const auto error = sink_(slot_, logicalToPhysical_);
+    if (!error.empty()) {
+      std::swap(row, logicalToPhysical_);
+      (void)sink_(slot_, logicalToPhysical_);
+      return error;
+    }
+  }
+  for (std::size_t i = lead; i < allocated; ++i) pool_->releasePage(row[i]);
+  currentLength_ = length;
+  return {};
 }
 
 std::string KVCacheState::reset() {

@@ -15,7 +15,12 @@
 //   * the block table is one device array [slots][maxPagesPerSequence] that
 //     decode kernels index; stageLength writes this sequence's row through a
 //     BlockTableSink instead of a per-request Metal buffer;
-//   * a contiguous (non-paged) cache is the pool with page size = capacity.
+//   * a contiguous (non-paged) cache is the pool with page size = capacity;
+//   * a page may belong to several sequences (forks of one prompt): the pool
+//     counts its owners and frees it with the last one. A sequence writes only
+//     into pages of its own: a fork gets a copy of the partly filled last page,
+//     and a sequence rolled back into a shared page replaces it by a copy
+//     before it appends (unshareTail).
 #pragma once
 
 #include <cstddef>
@@ -34,8 +39,8 @@ class KVPagePool {
   KVPagePool &operator=(const KVPagePool &) = delete;
 
   [[nodiscard]] std::size_t pageSize() const noexcept { return pageSize_; }
-  [[nodiscard]] std::size_t capacityPages() const noexcept { return allocated_.size(); }
-  [[nodiscard]] std::size_t usedPages() const noexcept { return allocated_.size() - freePages_.size(); }
+  [[nodiscard]] std::size_t capacityPages() const noexcept { return owners_.size(); }
+  [[nodiscard]] std::size_t usedPages() const noexcept { return owners_.size() - freePages_.size(); }
   [[nodiscard]] std::size_t availablePages() const noexcept { return freePages_.size(); }
   [[nodiscard]] std::size_t peakUsedPages() const noexcept { return peakUsedPages_; }
   [[nodiscard]] std::size_t allocationCount() const noexcept { return allocationCount_; }
@@ -44,8 +49,12 @@ class KVPagePool {
 
   // -1 when the pool is exhausted.
   [[nodiscard]] std::int32_t allocatePage();
-  // Throws std::invalid_argument for a page that is not allocated.
+  // One owner less; the last one frees the page. Throws std::invalid_argument
+  // for a page that is not allocated.
   void releasePage(std::int32_t page);
+  // One owner more. Throws std::invalid_argument for a page that is not allocated.
+  void retainPage(std::int32_t page);
+  [[nodiscard]] std::size_t owners(std::int32_t page) const noexcept;
 
   // Test hook: the next `n` allocations fail as if the pool were exhausted
   // (host-side failure injection; no device involvement).
@@ -54,11 +63,17 @@ class KVPagePool {
  private:
   std::size_t pageSize_;
   std::vector<std::int32_t> freePages_;
-  std::vector<bool> allocated_;
+  std::vector<std::uint32_t> owners_;  // 0: free
   std::size_t peakUsedPages_ = 0;
   std::size_t allocationCount_ = 0;
   std::size_t releaseCount_ = 0;
   std::size_t injectedFailures_ = 0;
+};
+
+// A page whose contents are to be copied to another.
+struct KVPageCopy {
+  std::int32_t from;
+  std::int32_t to;
 };
 
 // Receives a sequence's block-table row whenever its page list changes.
@@ -88,6 +103,16 @@ class KVCacheState {
   [[nodiscard]] std::string rollbackLength(std::size_t length);
   // Throws std::invalid_argument for 0 or > capacity (KVCacheState.cpp:242-247).
   void commitLength(std::size_t length);
+  // Become a fork of `source` (this state must be empty): share its full pages
+  // and take a page for the partly filled one, which the caller then copies
+  // (appended to `copies`). All or nothing.
+  [[nodiscard]] std::string fork(const KVCacheState &source, std::vector<KVPageCopy> *copies);
+  // Before positions are appended: when the page that the next one falls into
+  // is shared, take one of its own for it, to be copied by the caller.
+  [[nodiscard]] std::string unshareTail(std::vector<KVPageCopy> *copies);
+  // Keep the first `lead` pages, put `pages` (allocated by the caller) behind
+  // them in place of the others and commit `length`. On failure nothing changes.
+  [[nodiscard]] std::string replaceTail(std::size_t lead, const std::vector<std::int32_t> &pages, std::size_t length);
   // Release every page and set the length to 0.
   [[nodiscard]] std::string reset();
 

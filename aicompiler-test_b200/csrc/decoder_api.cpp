@@ -436,6 +436,42 @@ int tmc_decoder_attach_local_peers(tmc_decoder *dec, tmc_decoder *const *ranks, 
   return done(dec->ex->attachLocalPeers(ex, rank));
 }
 
+int tmc_decoder_set_window(tmc_decoder *dec, int window, int sinks) {
+  if (!bind(dec)) return fail(TMC_ERR_INVALID, "null decoder");
+  return done(dec->ex->setWindow(window, sinks));
+}
+
+int tmc_decoder_fork(tmc_decoder *dec, int slot, const int32_t *slots, int count) {
+  if (!bind(dec) || slots == nullptr) return fail(TMC_ERR_INVALID, "null argument");
+  return done(dec->ex->forkSlot(slot, slots, count));
+}
+
+int tmc_decoder_compact(tmc_decoder *dec, int slot, const int32_t *keep, int count) {
+  if (!bind(dec) || keep == nullptr) return fail(TMC_ERR_INVALID, "null argument");
+  return done(dec->ex->compactSlot(slot, keep, count));
+}
+
+static int score_arguments(tmc_decoder *dec, int top, const int32_t *top_ids, const float *top_logprobs) {
+  if (!bind(dec)) return fail(TMC_ERR_INVALID, "null decoder");
+  if (top < 0 || top > 32 || top > dec->ex->config().vocab)
+    return fail(TMC_ERR_UNSUPPORTED, "token scores: top must be in [0, 32] and at most the vocabulary");
+  if (top > 0 && (top_ids == nullptr || top_logprobs == nullptr)) return fail(TMC_ERR_INVALID, "null argument");
+  return TMC_OK;
+}
+
+int tmc_decoder_score(tmc_decoder *dec, int slot, const int32_t *tokens, int count, float *logprobs, float *entropy,
+                      int32_t *ranks, int top, int32_t *top_ids, float *top_logprobs, int32_t *next_token) {
+  if (tokens == nullptr) return fail(TMC_ERR_INVALID, "null argument");
+  if (const int e = score_arguments(dec, top, top_ids, top_logprobs); e != TMC_OK) return e;
+  return done(dec->ex->score(slot, tokens, count, {logprobs, entropy, ranks, top, top_ids, top_logprobs}, next_token));
+}
+
+int tmc_decoder_token_logprobs(tmc_decoder *dec, const int32_t *targets, int rows, float *logprobs, float *entropy,
+                               int32_t *ranks, int top, int32_t *top_ids, float *top_logprobs) {
+  if (const int e = score_arguments(dec, top, top_ids, top_logprobs); e != TMC_OK) return e;
+  return done(dec->ex->tokenScores(targets, rows, {logprobs, entropy, ranks, top, top_ids, top_logprobs}));
+}
+
 int tmc_decoder_set_wait_budgets(tmc_decoder *dec, uint64_t peer_wait_ns, uint64_t local_wait_ns) {
   if (!bind(dec)) return fail(TMC_ERR_INVALID, "null decoder");
   return done(dec->ex->setWaitBudgets(peer_wait_ns, local_wait_ns));

@@ -759,6 +759,12 @@ size_t window_attention_workspace_bytes(int sequences, int max_rows, int hq, int
   return partial_bytes(sequences, max_rows, hq, d, plan.outer);
 }
 
+int window_attention_launches(int sequences, int max_rows, int hq, int hkv, int d, long long window, long long sinks,
+                              long long capacity, int num_sms) {
+  const long long keys = visible_bound(window, sinks, max_rows, capacity);
+  return make_plan(sequences, max_rows, hq, hkv, d, keys, num_sms).outer > 1 ? 2 : 1;
+}
+
 cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, int num_sms, cudaStream_t stream,
                                     bool pdl) {
   if (p.sequences <= 0 || p.sequences > 65535 || p.rows < 0 || p.max_rows <= 0 || p.hkv <= 0 || p.hq <= 0 ||

@@ -38,6 +38,10 @@ struct WindowAttentionParams {
 size_t window_attention_workspace_bytes(int sequences, int max_rows, int hq, int hkv, int d, long long window,
                                         long long sinks, int num_sms);
 
+// Kernels that a launch with that workspace is made of (1 or 2).
+int window_attention_launches(int sequences, int max_rows, int hq, int hkv, int d, long long window, long long sinks,
+                              long long capacity, int num_sms);
+
 // fp16, or bf16 when `bf16`; d 16, 32, 64 or 128; q_stride and out_stride
 // multiples of 8, q, out and the pools 16-byte aligned.
 cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, int num_sms, cudaStream_t stream,

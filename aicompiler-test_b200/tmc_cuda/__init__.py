@@ -560,6 +560,13 @@ _sig("tmc_decoder_exchange_handle", c_int, c_void_p, ctypes.c_char_p, c_size_t)
 _sig("tmc_decoder_attach_peers", c_int, c_void_p, ctypes.c_char_p, c_size_t, c_int, c_int)
 _sig("tmc_decoder_attach_local_peers", c_int, c_void_p, POINTER(c_void_p), c_int, c_int)
 _sig("tmc_decoder_set_wait_budgets", c_int, c_void_p, c_uint64, c_uint64)
+_sig("tmc_decoder_set_window", c_int, c_void_p, c_int, c_int)
+_sig("tmc_decoder_fork", c_int, c_void_p, c_int, _I32P, c_int)
+_sig("tmc_decoder_compact", c_int, c_void_p, c_int, _I32P, c_int)
+_sig("tmc_decoder_score", c_int, c_void_p, c_int, _I32P, c_int, POINTER(c_float), POINTER(c_float), _I32P, c_int, _I32P,
+     POINTER(c_float), _I32P)
+_sig("tmc_decoder_token_logprobs", c_int, c_void_p, _I32P, c_int, POINTER(c_float), POINTER(c_float), _I32P, c_int,
+     _I32P, POINTER(c_float))
 EXCHANGE_HANDLE_BYTES = 64
 
 
@@ -913,6 +920,50 @@ class Decoder:
         check(lib.tmc_decoder_block_table(self.handle, slot, None, 0, ctypes.byref(n)))
         out = np.zeros(n.value, np.int32)
         check(lib.tmc_decoder_block_table(self.handle, slot, out.ctypes.data_as(_I32P), n.value, ctypes.byref(n)))
+        return out
+
+    def set_window(self, window, sinks=0):
+        """Attend to the newest `window` positions and the first `sinks` (0: to all)."""
+        check(lib.tmc_decoder_set_window(self.handle, window, sinks))
+
+    def fork(self, slot, slots):
+        """Make the empty `slots` forks of `slot` (shared full pages)."""
+        s = _i32(slots)
+        check(lib.tmc_decoder_fork(self.handle, slot, s.ctypes.data_as(_I32P), s.size))
+
+    def compact(self, slot, keep):
+        """Keep only the positions `keep` (ascending) of a sequence, moved together."""
+        k = _i32(keep)
+        check(lib.tmc_decoder_compact(self.handle, slot, k.ctypes.data_as(_I32P), k.size))
+
+    @staticmethod
+    def _score_arrays(rows, top):
+        return {"logprobs": np.empty(rows, np.float32), "entropy": np.empty(rows, np.float32),
+                "ranks": np.empty(rows, np.int32), "top_ids": np.empty((rows, top), np.int32),
+                "top_logprobs": np.empty((rows, top), np.float32)}
+
+    @staticmethod
+    def _score_pointers(a, top):
+        return (_fptr(a["logprobs"]), _fptr(a["entropy"]), a["ranks"].ctypes.data_as(_I32P), top,
+                a["top_ids"].ctypes.data_as(_I32P), _fptr(a["top_logprobs"]))
+
+    def score(self, tokens, slot=0, top=0):
+        """Prefill that scores every position's next token on the GPU: (arrays, next token)."""
+        t = _i32(tokens)
+        out = self._score_arrays(t.size, top)
+        nxt = np.zeros(1, dtype=np.int32)
+        check(lib.tmc_decoder_score(self.handle, slot, t.ctypes.data_as(_I32P), t.size, *self._score_pointers(out, top),
+                                    nxt.ctypes.data_as(_I32P)))
+        return out, int(nxt[0])
+
+    def token_logprobs(self, rows, targets=None, top=0):
+        """Scores of `targets` (None: the greedy tokens) under the last step's logits."""
+        t = None if targets is None else _i32(targets)
+        if t is not None and t.size != rows:
+            raise ValueError("one target per row")
+        out = self._score_arrays(rows, top)
+        check(lib.tmc_decoder_token_logprobs(self.handle, None if t is None else t.ctypes.data_as(_I32P), rows,
+                                             *self._score_pointers(out, top)))
         return out
 
     def stage(self, slot, length):

@@ -611,6 +611,37 @@ int tmc_decoder_attach_peers(tmc_decoder *dec, const uint8_t *handles, size_t nb
  * (ranks[rank] == dec), each on a device with peer access to dec's; their
  * windows are used directly. Each rank attaches once. */
 int tmc_decoder_attach_local_peers(tmc_decoder *dec, tmc_decoder *const *ranks, int world, int rank);
+/* Sliding window: from now on the queries of this decoder attend to the newest
+ * `window` positions (their own included) and to the first `sinks` positions of
+ * their sequence (tmc_k_window_attention's rule). 0: all positions, the state
+ * after creation. Positions keep their cache rows; to free rows, and to go on
+ * beyond the capacity, drop positions with tmc_decoder_compact. */
+int tmc_decoder_set_window(tmc_decoder *dec, int window, int sinks);
+
+/* Make every slot of `slots` (empty, distinct) a fork of `slot`: the pages that
+ * its committed positions fill are shared until their last owner lets them go,
+ * a partly filled last page is copied. The forks then go their own ways. */
+int tmc_decoder_fork(tmc_decoder *dec, int slot, const int32_t *slots, int count);
+
+/* Keep only the committed positions keep[0 .. count) (ascending) of a sequence:
+ * kept row i becomes position i, its key turned back by the distance moved
+ * (tmc_k_kv_compact), and the length `count`. Needs free pages for the rows that
+ * move before the old ones are freed; on failure the sequence is unchanged. */
+int tmc_decoder_compact(tmc_decoder *dec, int slot, const int32_t *keep, int count);
+
+/* tmc_decoder_prefill that scores the prompt on the GPU instead of returning
+ * logits: for position i the log probability, entropy and rank of tokens[i + 1]
+ * and the `top` (0 .. 32) largest alternatives, as tmc_k_token_logprobs gives
+ * them ([count] and [count, top] host arrays; NULL ones are left out; the last
+ * position has no next token: 0 and -1). One rank only (no tensor parallelism). */
+int tmc_decoder_score(tmc_decoder *dec, int slot, const int32_t *tokens, int count, float *logprobs, float *entropy,
+                      int32_t *ranks, int top, int32_t *top_ids, float *top_logprobs, int32_t *next_token);
+/* The same for targets[r] (NULL: the greedy tokens) under row r of the last
+ * step's logits: the rows of the last decode or generate call, or of a
+ * prefill's last chunk. */
+int tmc_decoder_token_logprobs(tmc_decoder *dec, const int32_t *targets, int rows, float *logprobs, float *entropy,
+                               int32_t *ranks, int top, int32_t *top_ids, float *top_logprobs);
+
 /* Budgets of the decoder kernels' bounded waits, in ns of global time (0: the
  * defaults, 10 s for another rank's exchange flags and 1 s for the tensor-core
  * GEMM's mbarrier and split-tile waits). A wait that runs out is recorded in
