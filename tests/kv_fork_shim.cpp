@@ -1,5 +1,5 @@
 // Test-only additions to kv_state_shim.cpp: forks, copies before appends and
-// replaced pages of the cache state (tests/test_kv_fork.py).
+// replaced pages of the cache state (tests/test_cache_fork.py).
 #include "kv_state_shim.cpp"
 
 extern "C" {
