@@ -160,7 +160,8 @@ template <typename T>
 struct Pass {
   using L = Logit<T>;
   static constexpr int N = L::kVec;
-  float m = -INFINITY, s[4] = {}, u[4] = {};
+  float m = -INFINITY;
+  float2 s[2] = {}, u[2] = {};
   float before = 0.0f;     // logits before the target: a whole number below 2^24
   float best = -INFINITY;  // the largest logit, and the first index of the vector that holds it
   int best_at = -1;
@@ -178,25 +179,28 @@ struct Pass {
       if (m != -INFINITY) {
         const float d = fmaxf(m - mx, -1e30f), f = exp2f(d * kLog2e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          u[i] = fmaf(s[i], d, u[i]) * f;
-          s[i] *= f;
+        for (int i = 0; i < 2; ++i) {
+          u[i] = make_float2(fmaf(s[i].x, d, u[i].x) * f, fmaf(s[i].y, d, u[i].y) * f);
+          s[i] = make_float2(s[i].x * f, s[i].y * f);
         }
       }
       m = mx;
     }
   }
-  __device__ __forceinline__ void weigh(float x, float about, int i) {
+  // Two logits at once (packed fp32 arithmetic) into partial sums i.
+  __device__ __forceinline__ void weigh(float x0, float x1, float about, int i) {
     // A masked logit (-inf) or one far below the maximum: 0 times a finite number.
-    const float d = max_or_nan(x - about, -1e4f);
-    const float e = exp2_fast(d * kLog2e);
-    s[i & 3] += e;
-    u[i & 3] = fmaf(e, d, u[i & 3]);
+    float2 d = __fadd2_rn(make_float2(x0, x1), make_float2(-about, -about));
+    d = make_float2(max_or_nan(d.x, -1e4f), max_or_nan(d.y, -1e4f));
+    const float2 t = __fmul2_rn(d, make_float2(kLog2e, kLog2e));
+    const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+    s[i & 1] = __fadd2_rn(s[i & 1], e);
+    u[i & 1] = __ffma2_rn(e, d, u[i & 1]);
   }
   // One logit.
   __device__ __forceinline__ void take(float x, int at, float xt, int target) {
     raise(x, at);
-    weigh(x, m == -INFINITY ? 0.0f : m, 0);
+    weigh(x, -INFINITY, m == -INFINITY ? 0.0f : m, 0);  // -inf weighs nothing
     before += (x > xt || (x == xt && at < target)) ? 1.0f : 0.0f;
   }
   // V vectors, `step` vectors apart, the first at index `at`.
@@ -213,7 +217,7 @@ struct Pass {
       float x[N];
       L::unpack(raw[v], x);
 #pragma unroll
-      for (int i = 0; i < N; ++i) weigh(x[i], about, i);
+      for (int i = 0; i < N; i += 2) weigh(x[i], x[i + 1], about, i / 2);
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -231,7 +235,7 @@ struct Pass {
     }
   }
   __device__ __forceinline__ Stats stats() const {
-    return {m, (s[0] + s[1]) + (s[2] + s[3]), (u[0] + u[1]) + (u[2] + u[3])};
+    return {m, (s[0].x + s[0].y) + (s[1].x + s[1].y), (u[0].x + u[0].y) + (u[1].x + u[1].y)};
   }
 };
 
