@@ -71,6 +71,16 @@ __device__ __forceinline__ void tmem_load128(uint32_t at, float *v) {
 #pragma unroll
   for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_load32(uint32_t at, float *v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_load16(uint32_t at, float *v) {
   uint32_t r[16];
   asm volatile(
@@ -371,10 +381,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             load(x);
             continue;
           }
-          float mx = -INFINITY;
+          float y[8];
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) mx = fmaxf(mx, x[i]);
-          mx *= scale;
+          for (int i = 0; i < 8; ++i) y[i] = x[i];
+#pragma unroll
+          for (int i = 8; i < kKeys; ++i) y[i % 8] = fmaxf(y[i % 8], x[i]);
+          const float mx = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                                 fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))) * scale;
           rise = rise && mx > m_run;
           const float f = rise ? exp2_fast(m_run - mx) : 1.0f;
 #pragma unroll
@@ -452,11 +465,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int part = 0; part < 2; ++part) {  // D / 2 fp32 columns fill a row's place
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
-              float x[16];
-              tmem_load16(o_at + part * (D / 2) + c, x);
+            for (int c = 0; c < D / 2; c += 32) {
+              float x[32];
+              tmem_load32(o_at + part * (D / 2) + c, x);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
+              for (int i = 0; i < 8; ++i)
                 *reinterpret_cast<float4 *>(own_rows + swizzled(r, c / 4 + i)) =
                     make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
@@ -464,11 +477,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            float x[16];
-            tmem_load16(o_at + c, x);
+          for (int c = 0; c < D; c += 32) {
+            float x[32];
+            tmem_load32(o_at + c, x);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 4; ++i)
               *reinterpret_cast<uint4 *>(own_rows + swizzled(r, c / 8 + i)) =
                   make_uint4(pack2(x[8 * i] * inv, x[8 * i + 1] * inv, E()),
                              pack2(x[8 * i + 2] * inv, x[8 * i + 3] * inv, E()),
