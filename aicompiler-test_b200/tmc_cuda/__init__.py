@@ -429,6 +429,7 @@ def paged_attention_f16(rt: Runtime, q: Buffer, out: Buffer, k_pool: Buffer, v_p
 # one by one costs more than the launch.
 
 _ELEMENT_TYPES = {F16: F16, F32: F32, BF16: BF16, I32: I32}
+_KNOWN = {code: {code} for code in _ELEMENT_TYPES}  # the spellings of a type met so far
 _FOREIGN_TYPES = {"float16": F16, "float32": F32, "bfloat16": BF16, "int32": I32}
 _window_attention_slots = struct.Struct("=23qf4x4q").pack
 _token_logprobs_slots = struct.Struct("=14q").pack
@@ -439,8 +440,20 @@ _kv_compact_slots = struct.Struct("=19q").pack
 def _element_type(dtype) -> int:
     code = _ELEMENT_TYPES.get(dtype)
     if code is None:
-        code = _ELEMENT_TYPES[dtype] = _FOREIGN_TYPES[str(dtype).rpartition(".")[2]]
+        name = str(dtype).rpartition(".")[2]
+        if name not in _FOREIGN_TYPES:
+            raise TypeError(f"arrays of {name} are not supported")
+        code = _ELEMENT_TYPES[dtype] = _FOREIGN_TYPES[name]
+        _KNOWN[code].add(dtype)
     return code
+
+
+def _expect(want: int, dtypes: set):
+    """Arrays of these types hold elements `want` all: the kernels cannot tell."""
+    if not dtypes <= _KNOWN[want]:
+        for dtype in dtypes:
+            if _element_type(dtype) != want:
+                raise TypeError(f"an array of {dtype} where element type {want} (F16, F32, BF16, I32 = 0 .. 3) is expected")
 
 
 def _address(array) -> int:
@@ -459,9 +472,12 @@ def window_attention(rt: Runtime, q, out, k_pool, v_pool, block_table, table_str
                      q_stride: int | None = None, out_stride: int | None = None, workspace=None, stream=None):
     """Attention over the paged cache with a sliding window and `sinks` first positions that
     stay visible, for ragged query rows (tmc_k_window_attention); fp16 or bf16, as q."""
+    dtype = _element_type(q.dtype)
+    _expect(dtype, {out.dtype, k_pool.dtype, v_pool.dtype})
+    _expect(I32, {block_table.dtype, table_rows.dtype, row_starts.dtype, first_positions.dtype})
     code = lib.tmc_k_window_attention_slots(_window_attention_slots(
         q.data_ptr(), hq * d if q_stride is None else q_stride, out.data_ptr(),
-        hq * d if out_stride is None else out_stride, k_pool.data_ptr(), v_pool.data_ptr(), _element_type(q.dtype),
+        hq * d if out_stride is None else out_stride, k_pool.data_ptr(), v_pool.data_ptr(), dtype,
         block_table.data_ptr(), table_stride, table_rows.data_ptr(), row_starts.data_ptr(), first_positions.data_ptr(),
         sequences, rows, max_rows, hq, hkv, d, page_size, pool_pages, capacity, window, sinks, scale,
         _address(workspace), 0 if workspace is None else workspace.nbytes, rt.status_ptr or 0,
@@ -474,6 +490,8 @@ def token_logprobs(rt: Runtime, logits, targets, rows: int, vocab: int, logprobs
                    top: int = 0, top_ids=None, top_logprobs=None, row_stride: int | None = None, stream=None):
     """Log probability, rank and entropy of one given token per row of logits, with the `top`
     largest alternatives (tmc_k_token_logprobs)."""
+    _expect(I32, {x.dtype for x in (targets, ranks, top_ids) if x is not None})
+    _expect(F32, {x.dtype for x in (logprobs, entropy, top_logprobs) if x is not None})
     code = lib.tmc_k_token_logprobs_slots(_token_logprobs_slots(
         logits.data_ptr(), _element_type(logits.dtype), vocab if row_stride is None else row_stride, _address(targets),
         rows, vocab, _address(logprobs), _address(entropy), _address(ranks), top, _address(top_ids) if top else 0,
@@ -486,6 +504,7 @@ def kv_copy_pages(rt: Runtime, pools, pool_count: int, pool_pages: int, page_byt
                   stream=None):
     """Copy page src[i] to page dst[i] of every pool; pools: device array of addresses
     (tmc_k_kv_copy_pages)."""
+    _expect(I32, {src.dtype, dst.dtype})
     code = lib.tmc_k_kv_copy_pages_slots(_kv_copy_pages_slots(
         pools.data_ptr(), pool_count, pool_pages, page_bytes, src.data_ptr(), dst.data_ptr(), count,
         rt.status_ptr or 0, (rt.stream if stream is None else stream) or 0))
@@ -498,6 +517,8 @@ def kv_compact(rt: Runtime, pools, layers: int, pool_pages: int, hkv: int, d: in
                rope_sin=None, rope_rows: int = 0, dtype: int = F16, stream=None):
     """Move the kept rows of a sequence together into other pages, keys turned by the distance
     moved (tmc_k_kv_compact)."""
+    _expect(I32, {src_pages.dtype, dst_pages.dtype, keep.dtype})
+    _expect(F32, {x.dtype for x in (rope_cos, rope_sin) if x is not None})
     code = lib.tmc_k_kv_compact_slots(_kv_compact_slots(
         pools.data_ptr(), layers, dtype, pool_pages, hkv, d, page_size, src_pages.data_ptr(), src_count,
         dst_pages.data_ptr(), dst_count, keep.data_ptr(), count, first, _address(rope_cos), _address(rope_sin),

@@ -286,7 +286,8 @@ int tmc_k_paged_attention_f16_noalloc(const void *q, void *out, const void *k_po
  * the keys j <= p with p - j < window or j < sinks (window >= capacity: all
  * earlier keys).
  *   q, out   rows of [hq, d], q_stride / out_stride elements from row to row
- *            (multiples of 8, at least hq * d), fp16 or bf16 (dtype)
+ *            (multiples of 8, at least hq * d), fp16 or bf16 (dtype); out may
+ *            be q, with the same stride
  *   k_pool,
  *   v_pool   [pool_pages, hkv, page_size, d], any page_size >= 1, same dtype
  *   block_table [.., table_stride] int32, row table_rows[s] for sequence s;

@@ -111,23 +111,66 @@ def test_integers_beyond_32_bits_are_refused():
     class Runtime:
         stream = status_ptr = None
 
-    a, rt = Array(), Runtime()
+    a, n, f, rt = Array(), Array(tmc_cuda.I32), Array(tmc_cuda.F32), Runtime()
     with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
-        tmc_cuda.window_attention(rt, a, a, a, a, a, 4, a, a, a, 1, 1, 1, 4, 2, 128, 16, 8, 64, 1 << 32, 0)
+        tmc_cuda.window_attention(rt, a, a, a, a, n, 4, n, n, n, 1, 1, 1, 4, 2, 128, 16, 8, 64, 1 << 32, 0)
     with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
-        tmc_cuda.kv_copy_pages(rt, a, 2, 8, 64, a, a, (1 << 32) + 1)
+        tmc_cuda.kv_copy_pages(rt, a, 2, 8, 64, n, n, (1 << 32) + 1)
     with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
-        tmc_cuda.token_logprobs(rt, a, a, 1 << 33, 100, a)
+        tmc_cuda.token_logprobs(rt, a, n, 1 << 33, 100, f)
     with pytest.raises(tmc_cuda.TmcError, match="32 bits"):
-        tmc_cuda.kv_compact(rt, a, 1, 8, 2, 64, 16, a, 4, a, 4, a, 1 << 32)
+        tmc_cuda.kv_compact(rt, a, 1, 8, 2, 64, 16, n, 4, n, 4, n, 1 << 32)
     # the same refusals as the C entries give, through the packed form
     with pytest.raises(tmc_cuda.TmcError, match="window >= 1"):
-        tmc_cuda.window_attention(rt, a, a, a, a, a, 4, a, a, a, 1, 1, 1, 4, 2, 128, 16, 8, 64, 0, 0)
+        tmc_cuda.window_attention(rt, a, a, a, a, n, 4, n, n, n, 1, 1, 1, 4, 2, 128, 16, 8, 64, 0, 0)
     with pytest.raises(tmc_cuda.TmcError, match="scale"):
-        tmc_cuda.window_attention(rt, a, a, a, a, a, 4, a, a, a, 1, 1, 1, 4, 2, 128, 16, 8, 64, 9, 0, scale=-0.5)
+        tmc_cuda.window_attention(rt, a, a, a, a, n, 4, n, n, n, 1, 1, 1, 4, 2, 128, 16, 8, 64, 9, 0, scale=-0.5)
     with pytest.raises(tmc_cuda.TmcError, match="top"):
-        tmc_cuda.token_logprobs(rt, a, a, 1, 100, a, top=33, top_ids=a, top_logprobs=a)
+        tmc_cuda.token_logprobs(rt, a, n, 1, 100, f, top=33, top_ids=n, top_logprobs=f)
     with pytest.raises(tmc_cuda.TmcError, match="multiple of 8"):
-        tmc_cuda.kv_compact(rt, a, 1, 8, 2, 12, 16, a, 4, a, 4, a, 1)
+        tmc_cuda.kv_compact(rt, a, 1, 8, 2, 12, 16, n, 4, n, 4, n, 1)
     for name in ("window_attention", "token_logprobs", "kv_copy_pages", "kv_compact"):
         assert getattr(tmc_cuda.lib, f"tmc_k_{name}_slots")(None) == tmc_cuda.ERR_INVALID
+
+
+class Array:
+    """Stands for a tensor of another library; nothing reads its memory."""
+
+    def __init__(self, dtype):
+        self.dtype, self.nbytes = dtype, 64
+
+    def data_ptr(self):
+        return P
+
+
+class Handles:
+    stream = status_ptr = None
+
+
+@pytest.mark.parametrize("wrong", ["out", "k", "table", "starts"])
+def test_attention_arrays_of_another_type_are_refused(wrong):
+    types = dict(q="torch.float16", out="torch.float16", k="torch.float16", v="torch.float16", table="torch.int32",
+                 rows="torch.int32", starts="torch.int32", first="torch.int32")
+    types[wrong] = "torch.bfloat16" if types[wrong] == "torch.float16" else "torch.int64"
+    a = {k: Array(t) for k, t in types.items()}
+    with pytest.raises(TypeError):
+        tmc_cuda.window_attention(Handles, a["q"], a["out"], a["k"], a["v"], a["table"], 4, a["rows"], a["starts"],
+                                  a["first"], 0, 0, 1, 4, 2, 128, 16, 8, 64, 16)
+
+
+def test_other_arrays_of_another_type_are_refused():
+    f, i, wide = Array("torch.float32"), Array("torch.int32"), Array("torch.int64")
+    with pytest.raises(TypeError):  # token ids as they come from an embedding's input
+        tmc_cuda.token_logprobs(Handles, f, wide, 0, 100, f)
+    with pytest.raises(TypeError):
+        tmc_cuda.token_logprobs(Handles, f, i, 0, 100, Array("torch.bfloat16"))
+    with pytest.raises(TypeError):
+        tmc_cuda.token_logprobs(Handles, wide, i, 0, 100, f)
+    with pytest.raises(TypeError):
+        tmc_cuda.token_logprobs(Handles, Array("torch.float64"), i, 0, 100, f)
+    with pytest.raises(TypeError):
+        tmc_cuda.kv_copy_pages(Handles, wide, 2, 8, 64, wide, i, 0)
+    with pytest.raises(TypeError):
+        tmc_cuda.kv_compact(Handles, wide, 1, 8, 2, 64, 16, i, 4, i, 4, wide, 0)
+    tmc_cuda.token_logprobs(Handles, f, i, 0, 100, f)
+    tmc_cuda.kv_copy_pages(Handles, wide, 2, 8, 64, i, i, 0)
