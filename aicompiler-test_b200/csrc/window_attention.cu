@@ -1,17 +1,22 @@
 // Window attention with sinks over the paged cache (window_attention.cuh).
 //
-// Both kernels make one pass over the visible keys with a running maximum and
-// sum per query row: S = scale log2(e) Q K^T, p = 2^(S - m), O += P V, and
-// O / l at the end, S and O in fp32, products by mma.sync m16n8k16. The G = Hq /
-// Hkv query heads of a KV head are rows of the same tile, so a key is read
-// once for all of them. The visible keys of a tile are numbered without a gap:
-// the sinks before the window, then the window's run.
+// One pass over the visible keys with a running maximum and sum per query row:
+// S = scale log2(e) Q K^T, p = 2^(S - m), O += P V, and O / l at the end, S and
+// O in fp32. The G = Hq / Hkv query heads of a KV head are rows of the same
+// tile, so a key is read once for all of them. The visible keys of a tile are
+// numbered without a gap: the sinks before the window, then the window's run.
 //
-// - decode (one row per sequence): a warp takes 16 keys at a time through a
-//   ring of its own, with no barrier between warps; the warps of a CTA, and
+// - decode (one row per sequence): bound by the reads of K and V, G products a
+//   key, so mma.sync m16n8k16 keeps up. A warp takes 16 keys at a time through
+//   a ring of its own, with no barrier between warps; the warps of a CTA, and
 //   the CTAs of a cluster, split the keys and join their states in shared and
-//   distributed shared memory.
-// - prompts: a CTA holds 128 query rows x heads, its warps 16 each, and all
+//   distributed shared memory. Heads of 128, 8 KV heads: 64 sequences of 700 to
+//   8192 positions, window 4096, 146 us (5.9 TB/s, 0.91 of a copy's rate); one
+//   sequence, window 1024, 7.0 us, which is launch, three dependent reads
+//   (sequence, table, keys) and the joins.
+// - prompts with heads of 64 and 128 run in window_tensor.cu. Short heads (16,
+//   32) have a quarter of the products or less per exponential and stay on
+//   mma.sync: a CTA holds 128 query rows x heads, its warps 16 each, and all
 //   share 64-key tiles.
 // When a launch has too few CTAs for the GPU its splits write their states to
 // the workspace, and a second kernel joins them.
@@ -28,9 +33,12 @@ namespace {
 
 using namespace window;
 
-constexpr int kMaxCluster = 8;    // CTAs of a decode cluster
-constexpr int kDecodePerSm = 3;  // decode CTAs that an SM holds
-constexpr int kMaxOuter = 32;    // splits that meet through the workspace
+constexpr int kMaxCluster = 8;   // CTAs of a decode cluster; 16 find room later and were slower
+// Decode CTAs that an SM holds, at 168 registers a thread. Two (with up to 255)
+// take one row of 1k keys in 6.5 us instead of 7.0, but keep fewer reads in
+// flight: one row of 32k keys 43 us instead of 30, three stages or not.
+constexpr int kDecodePerSm = 3;
+constexpr int kMaxOuter = 32;  // splits that meet through the workspace
 
 // Add a state's weighted part: ml its (maximum, sum), m the maximum over all.
 __device__ __forceinline__ void join_part(const float2 &ml, const float4 &x, float m, float &l, float4 &o) {
@@ -623,9 +631,12 @@ size_t partial_bytes(int sequences, int max_rows, int hq, int d, int outer) {
 Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long keys, int num_sms) {
   const int g = hq / hkv;
   Plan plan{max_rows == 1, max_rows > 1 && (d == 64 || d == 128), 1, 1, 1};
-  plan.tiles = plan.decode ? (g + 15) / 16 : (int)(((long long)max_rows * g + (plan.tensor ? 255 : 127)) / (plan.tensor ? 256 : 128));
+  const long long height = plan.tensor ? 256 : 128;  // tile rows of a prompt CTA
+  plan.tiles = plan.decode ? (g + 15) / 16 : (int)((max_rows * (long long)g + height - 1) / height);
   const long long ctas = (long long)sequences * hkv * plan.tiles;
   const long long slots = (plan.decode ? kDecodePerSm : plan.tensor ? 1 : 2) * num_sms;  // CTAs that run at the same time
+  // Tensor-core prompts: one round of CTAs, down to one step of 128 keys each
+  // (64 rows x 32 heads over 1000 keys 17.2 us; two steps at least 18.7).
   if (plan.tensor) {
     const long long steps = (keys + 127) / 128;
     long long splits = slots / ctas;
@@ -639,8 +650,10 @@ Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long ke
     return plan;
   }
   // Few CTAs: as many splits as run at once, each with one step of keys for
-  // its four warps at least. Many: a few rounds of CTAs, which evens out
-  // sequences of different lengths, each with eight steps at least.
+  // its four warps at least. Many: two and a half rounds of CTAs, which evens
+  // out sequences of different lengths, each with eight steps at least (64
+  // sequences of 700 .. 4100 keys: one round 161 us, two and a half 147, five
+  // 146; 128 of 100 .. 1000 keys: 65, 68, 79).
   long long splits;
   if (2 * ctas <= slots) {
     splits = slots / ctas;
@@ -650,7 +663,8 @@ Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long ke
     if (splits * 512 > keys) splits = (keys + 511) / 512;
   }
   // Beyond a cluster the splits' states meet in the workspace, at the cost of
-  // a second launch: that takes four clusters' worth of them, of 256 keys each.
+  // a second launch: that takes four clusters' worth of them, of 256 keys each
+  // (8 KV heads of one row over 32k keys: 30 us, in one cluster each 71).
   const long long wide = splits < keys / 256 ? splits : keys / 256;
   if (wide < 4 * kMaxCluster) {
     plan.cluster = (int)(splits < kMaxCluster ? splits : kMaxCluster);

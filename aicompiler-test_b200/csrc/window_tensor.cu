@@ -23,6 +23,19 @@
 // Values that are infinite or NaN in a step that some row does not wholly see
 // would reach that row as 0 x inf: such a step marks the tile, and the tile's
 // rows are computed again by plain loops.
+//
+// Bound: per 128 keys a tile's softmax takes 2140 cycles and its products 1330,
+// of which two tiles overlap most: 8192 rows x 32 heads of 128 causally 568 us,
+// 968 TFLOP/s, 0.58 of the library product's rate (the products alone 418 us of
+// 605 in an earlier version, the softmax alone 459). Measured and left out: two
+// threads a row (656 us against 620), P handed over in halves (614 against
+// 606), an eighth to a half of the exponentials as polynomials (636 to 651
+// against 598), steps of 64 keys with S double-buffered (820 against 606: a
+// product with N = 64 takes as long as with 128), the splits joined in clusters
+// (512 rows over 8k keys 84 us against 88, but 57 against 33 where clusters of
+// six leave SMs idle). Short calls are set-up and hand-over: 256 rows x 32
+// heads, window 512, 21 us, of which reading the first keys 4, a step 2, the
+// results 2 to 3 and the joining kernel 4.
 #include <map>
 #include <mutex>
 #include <utility>
@@ -273,7 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool used = m < total;
     const int row = used ? m / g : 0, head = h * g + (used ? m % g : 0), pos = seq.first + row;
     // Rows go to and from shared memory by whole warps, a few rows at a time
-    // (each thread its own row: 4 us more per CTA for Q, 2 for the results).
+    // (each thread its own row: Q 3100 to 9000 cycles instead of 1300 to 4700,
+    // the results 4500 instead of 3700).
     constexpr int kChunks = D / 8, kRows = 32 / kChunks;  // 16-byte chunks of a row; rows at a time
     unsigned char *own_rows = sQ + t * C::kTile;
     const int r0 = (warp & 3) * 32;
@@ -448,7 +462,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float l = (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
         // Q has been read: its place takes the results, 256-byte (D 64: 128-byte) pieces of each row.
-        const long long row_at = !used ? -1 : splits > 1 ? (split * slots + slot) * D : (seq.start + row) * p.out_stride + (long long)head * D;
+        const long long row_at = !used        ? -1
+                                 : splits > 1 ? (split * slots + slot) * D
+                                              : (seq.start + row) * p.out_stride + (long long)head * D;
         auto hand_out = [&](char *to, int size, int bytes_before) {  // the warp's 32 rows, chunks in order
           __syncwarp();
 #pragma unroll 4
