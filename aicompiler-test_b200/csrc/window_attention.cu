@@ -36,7 +36,7 @@ using namespace window;
 constexpr int kMaxCluster = 8;   // CTAs of a decode cluster; 16 find room later and were slower
 // Decode CTAs that an SM holds, at 168 registers a thread. Two (with up to 255)
 // take one row of 1k keys in 6.5 us instead of 7.0, but keep fewer reads in
-// flight: one row of 32k keys 43 us instead of 30, three stages or not.
+// flight: one row of 32k keys 37 us instead of 30, three stages or not.
 constexpr int kDecodePerSm = 3;
 constexpr int kMaxOuter = 32;  // splits that meet through the workspace
 
@@ -663,15 +663,19 @@ Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long ke
     if (splits * 512 > keys) splits = (keys + 511) / 512;
   }
   // Beyond a cluster the splits' states meet in the workspace, at the cost of
-  // a second launch: that takes four clusters' worth of them, of 256 keys each
-  // (8 KV heads of one row over 32k keys: 30 us, in one cluster each 71).
-  const long long wide = splits < keys / 256 ? splits : keys / 256;
-  if (wide < 4 * kMaxCluster) {
+  // a second launch: three clusters or more, of 128 keys a CTA at least, on
+  // seven eighths of the CTAs' places (clusters of eight do not fill the rest).
+  // 8 KV heads of one row over 4096 keys 9.8 us (in one cluster 13.2), of two
+  // rows over 16k 31 (46), over 2048 keys, where it takes one cluster, 8.8 (two
+  // 9.4); one KV head of two rows over 64k 24 us (on all places 30), of one row
+  // 16.1 (clusters of four 18.6).
+  const long long room = splits < 7 * slots / 8 / ctas ? splits : 7 * slots / 8 / ctas;
+  const long long wide = room < keys / 128 ? room : keys / 128;
+  if (wide < 3 * kMaxCluster) {
     plan.cluster = (int)(splits < kMaxCluster ? splits : kMaxCluster);
   } else {
-    splits = wide;
-    plan.cluster = kMaxCluster / 2;
-    plan.outer = (int)(splits / plan.cluster < kMaxOuter ? splits / plan.cluster : kMaxOuter);
+    plan.cluster = kMaxCluster;
+    plan.outer = (int)(wide / kMaxCluster < kMaxOuter ? wide / kMaxCluster : kMaxOuter);
   }
   return plan;
 }
