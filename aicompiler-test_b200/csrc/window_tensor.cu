@@ -244,8 +244,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int v = v0 + j * kKeys + lane * kBox;
     return lane < kKeys / kBox && j < steps && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
   };
-  KeyPlace first_box{0, -1, 0};
-  if (BOXES && warp >= kSoftmaxWarps && warp < kMmaWarp) first_box = find_box(0);  // on its way over the barrier
+  auto find_half = [&](int job, int i) {  // lane: key 32 i + lane of a half step; jobs K 0, K 1, V 0, V 1 of each step
+    const int v = v0 + (job >> 2) * kKeys + (job & 1) * 64 + i * 32 + lane;
+    return job < 4 * steps && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
+  };
+  // The first table entries are on their way over the barrier.
+  KeyPlace first_box{0, -1, 0}, first_half[2] = {{0, -1, 0}, {0, -1, 0}};
+  if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
+    if (BOXES) {
+      first_box = find_box(0);
+    } else {
+      first_half[0] = find_half(warp - kSoftmaxWarps, 0);
+      first_half[1] = find_half(warp - kSoftmaxWarps, 1);
+    }
+  }
 
   if (warp == kMmaWarp) {
     if (lane == 0) {
@@ -574,13 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- loads: the halves (64 keys) of K and of V of every step are dealt out
     // to the warps in the order in which they are needed ----
     const int load = warp - kSoftmaxWarps;
-    const int jobs = 4 * steps;  // per step: K 0, K 1, V 0, V 1
-    auto find = [&](int job, int i) {
-      const int v = v0 + (job >> 2) * kKeys + (job & 1) * 64 + i * 32 + lane;
-      return job < jobs && v < v1 ? find_key(p, seq.table, vis.key(v)) : KeyPlace{0, -1, 0};
-    };
-    KeyPlace next[2] = {find(load, 0), find(load, 1)};
-    for (int job = load; job < jobs; job += kLoadWarps) {
+    KeyPlace next[2] = {first_half[0], first_half[1]};
+    for (int job = load; job < 4 * steps; job += kLoadWarps) {
       const int j = job >> 2, st = j % S, half = job & 1;
       const bool value = (job & 2) != 0;
       uint32_t at[2];  // pool rows: below 2^32 for 128-byte rows of one GPU's memory; 0xffffffff: none
@@ -590,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int v = v0 + j * kKeys + half * 64 + i * 32 + lane;
         at[i] = v < v1 ? (uint32_t)pool_row(p, next[i], h, s) : 0xffffffffu;
         bad[i] = v < v1 && at[i] == 0xffffffffu;
-        next[i] = find(job + kLoadWarps, i);
+        next[i] = find_half(job + kLoadWarps, i);
       }
       uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
       if (j >= S && !__all_sync(0xffffffffu, wait(&empty[st], ((j / S) - 1) & 1))) {
