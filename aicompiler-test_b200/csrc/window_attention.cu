@@ -329,9 +329,8 @@ struct PromptCfg {
   static constexpr int kSmem = kStages * 2 * kStageBytes;
 };
 
-// Grid (splits x tiles, Hkv, sequences). Tile t holds the tile rows
-// t BM .. t BM + BM - 1 of the sequence's (row, head of the KV head) pairs,
-// heads fastest.
+// Grid as prompt_place counts it. Tile t holds the tile rows t BM .. t BM + BM - 1
+// of the sequence's (row, head of the KV head) pairs, heads fastest.
 template <typename E, int D>
 __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
     window_prompt_kernel(const WindowAttentionParams p, int splits) {
@@ -342,10 +341,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tq = lane & 3;
   pdl_wait();
-  const int s = blockIdx.z, h = blockIdx.y, split = blockIdx.x % splits;
-  const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
+  const PromptPlace place = prompt_place(p, splits);
+  const int s = place.seq, h = place.head, split = place.split;
+  const Sequence seq = load_sequence(p, s, place.first && tid == 0);
   const int g = p.hq / p.hkv;
-  const int m0 = (int)(blockIdx.x / splits) * C::BM, total = seq.rows * g;
+  const int m0 = place.tile * C::BM, total = seq.rows * g;
   if (m0 >= total) return;
   const int r_lo = m0 / g, r_hi = min(m0 + C::BM - 1, total - 1) / g;
   const int p_lo = seq.first + r_lo, p_hi = seq.first + r_hi;
@@ -710,6 +710,8 @@ cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t str
          (p.workspace == nullptr ||
           partial_bytes(p.sequences, p.max_rows, p.hq, D, plan.outer) > p.workspace_bytes))
     plan.outer /= 2;
+  if (!plan.decode && (long long)plan.tiles * plan.outer * p.hkv > 0x7fffffffll / p.sequences)
+    return cudaErrorInvalidValue;
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.stream = stream;
@@ -738,7 +740,7 @@ cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t str
   } else {
     const auto kernel = window_prompt_kernel<E, D>;
     if ((e = allow_smem(reinterpret_cast<const void *>(kernel), PromptCfg<D>::kSmem)) != cudaSuccess) return e;
-    cfg.gridDim = dim3((unsigned)(plan.tiles * plan.outer), p.hkv, p.sequences);
+    cfg.gridDim = dim3((unsigned)((long long)plan.tiles * plan.outer * p.hkv * p.sequences));
     cfg.blockDim = dim3(PromptCfg<D>::kThreads);
     cfg.dynamicSmemBytes = PromptCfg<D>::kSmem;
     add_pdl();

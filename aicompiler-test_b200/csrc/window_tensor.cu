@@ -25,9 +25,10 @@
 // rows are computed again by plain loops.
 //
 // Bound: per 128 keys a tile's softmax takes 2140 cycles and its products 1330,
-// of which two tiles overlap most: 8192 rows x 32 heads of 128 causally 568 us,
-// 968 TFLOP/s, 0.58 of the library product's rate (the products alone 418 us of
-// 605 in an earlier version, the softmax alone 459). Measured and left out: two
+// of which two tiles overlap most: 8192 rows x 32 heads of 128 causally 580 us,
+// 948 TFLOP/s, 0.57 of a library product's short-run rate and 0.69 of its rate
+// under the power limit (the products alone 418 us of 605 in an earlier version,
+// the softmax alone 459). Measured and left out: two
 // threads a row (656 us against 620), P handed over in halves (614 against
 // 606), an eighth to a half of the exponentials as polynomials (636 to 651
 // against 598), steps of 64 keys with S double-buffered (820 against 606: a
@@ -192,7 +193,7 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   return (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// Grid (splits x tile pairs, Hkv, sequences). BOXES: K and V by TMA boxes.
+// Grid as prompt_place counts it, over tile pairs. BOXES: K and V by TMA boxes.
 template <typename E, int D, bool BOXES>
 __global__ void __launch_bounds__(kThreads, 1)
     window_tensor_kernel(const WindowAttentionParams p, int splits, const __grid_constant__ CUtensorMap k_map,
@@ -212,11 +213,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (BOXES && tid < 2)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tid ? &v_map : &k_map)) : "memory");
   pdl_wait();
-  const int s = blockIdx.z, h = blockIdx.y, split = (gridDim.x - 1 - blockIdx.x) % splits;
-  const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
+  const PromptPlace place = prompt_place(p, splits);
+  const int s = place.seq, h = place.head, split = place.split;
+  const Sequence seq = load_sequence(p, s, place.first && tid == 0);
   const int g = p.hq / p.hkv;
-  // The last rows see the most keys: their tiles start first.
-  const int m0 = (int)((gridDim.x - 1 - blockIdx.x) / splits) * 2 * kTileRows, total = seq.rows * g;
+  const int m0 = place.tile * 2 * kTileRows, total = seq.rows * g;
   if (m0 >= total) return;
   const int tiles = m0 + kTileRows < total ? 2 : 1;
   const int m_end = min(m0 + 2 * kTileRows, total);
@@ -710,7 +711,7 @@ cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaSt
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(pairs * splits), p.hkv, p.sequences);
+  cfg.gridDim = dim3((unsigned)((long long)pairs * splits * p.hkv * p.sequences));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = TensorCfg<D>::kSmem;
   cfg.stream = stream;
