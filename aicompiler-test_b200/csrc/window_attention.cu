@@ -6,7 +6,7 @@
 // tile, so a key is read once for all of them. The visible keys of a tile are
 // numbered without a gap: the sinks before the window, then the window's run.
 //
-// - decode (one row per sequence): bound by the reads of K and V, G products a
+// - decode (one row per sequence, or few): bound by the reads of K and V, G products a
 //   key, so mma.sync m16n8k16 keeps up. A warp takes 16 keys at a time through
 //   a ring of its own, with no barrier between warps; the warps of a CTA, and
 //   the CTAs of a cluster, split the keys and join their states in shared and
@@ -14,6 +14,7 @@
 //   8192 positions, window 4096, 146 us (5.9 TB/s, 0.91 of a copy's rate); one
 //   sequence, window 1024, 7.0 us, which is launch, three dependent reads
 //   (sequence, table, keys) and the joins.
+//   Prompts of a few rows run the same way, each row with its own mask.
 // - prompts with heads of 64 and 128 run in window_tensor.cu. Short heads (16,
 //   32) have a quarter of the products or less per exponential and stay on
 //   mma.sync: a CTA holds 128 query rows x heads, its warps 16 each, and all
@@ -39,6 +40,13 @@ constexpr int kMaxCluster = 8;   // CTAs of a decode cluster; 16 find room later
 // flight: one row of 32k keys 37 us instead of 30, three stages or not.
 constexpr int kDecodePerSm = 3;
 constexpr int kMaxOuter = 32;  // splits that meet through the workspace
+// Prompts of at most 16 tile rows, or so short that all of their 16-row tiles
+// together read no more than this (elements of keys), run as decoding does: it
+// has less to set up, but reads the keys for every 16 rows. 32 heads, 8 KV heads
+// of 128: 2 rows over 1000 keys 7.7 us (as prompts 13.9), 16 rows 10.8 (14.6), 32
+// rows (8.5 million) 14.9 (15.0), 64 rows (17 million) 20.1 (17.1); 64 sequences
+// of 4 rows over 1000 to 2000 keys 100 us (131), 16 heads of 64 of their own 92 (211).
+constexpr long long kFewElements = 12500000;
 
 // Add a state's weighted part: ml its (maximum, sum), m the maximum over all.
 __device__ __forceinline__ void join_part(const float2 &ml, const float4 &x, float m, float &l, float4 &o) {
@@ -65,7 +73,7 @@ __device__ __forceinline__ void store_cluster(const float2 *local, int rank, flo
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(in_cta(local, rank)), "f"(a), "f"(b) : "memory");
 }
 
-// ---- decode: one row per sequence --------------------------------------------------------
+// ---- decode: one row per sequence, or a few ------------------------------------------------
 
 template <int D>
 struct DecodeCfg {
@@ -75,14 +83,17 @@ struct DecodeCfg {
   static constexpr int kRing = kWarps * kStages * 2 * kStageBytes;
   static constexpr int kMerge = kWarps * (16 * D + 32) * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
-  // and the parts that a cluster's CTAs send: a share each of `heads` rows
-  static constexpr int smem(int heads) { return kSmem + (heads * D + 4 * kMaxCluster) * 4; }
+  // and the parts that a cluster's CTAs send: a share each of `rows` tile rows
+  static constexpr int smem(int rows) { return kSmem + (rows * D + 4 * kMaxCluster) * 4; }
 };
 
-// Grid (splits, Hkv x head tiles, sequences), clusters of `cluster` CTAs along
-// the splits; outer = splits / cluster of them meet in the workspace.
-template <typename E, int D>
-__global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const WindowAttentionParams p, int head_tiles, int cluster) {
+// Grid (splits, Hkv x tiles, sequences), clusters of `cluster` CTAs along the
+// splits; outer = splits / cluster of them meet in the workspace. A tile is 16
+// of the (row, head of the KV head) pairs, heads fastest. ROWS: sequences may
+// have several rows, whose masks differ.
+template <typename E, int D, bool ROWS>
+__global__ void __launch_bounds__(128, kDecodePerSm)
+    window_decode_kernel(const WindowAttentionParams p, int tiles, int cluster) {
   using C = DecodeCfg<D>;
   constexpr int S = C::kStages;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -93,15 +104,18 @@ __global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const 
   const int gq = lane >> 2, tq = lane & 3;
   if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
-  const int s = blockIdx.z, h = blockIdx.y / head_tiles, tile = blockIdx.y % head_tiles;
+  const int s = blockIdx.z, h = blockIdx.y / tiles, m0 = blockIdx.y % tiles * 16;
   const int split = blockIdx.x, splits = gridDim.x;
   const Sequence seq = load_sequence(p, s, blockIdx.x == 0 && blockIdx.y == 0 && tid == 0);
-  if (seq.rows == 0) {  // the same for every CTA of the cluster
+  const int g = p.hq / p.hkv, used = min(16, seq.rows * g - m0);  // tile rows
+  if (used <= 0) {  // the same for every CTA of the cluster
     if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     return;
   }
-  const int g = p.hq / p.hkv, head0 = h * g + tile * 16, heads = min(16, g - tile * 16);
-  const Visible vis = visible_keys(p, seq.first, seq.first);
+  auto row_of = [&](int r) { return ROWS ? (m0 + r) / g : 0; };  // of tile row r
+  auto head_of = [&](int r) { return h * g + m0 + r - row_of(r) * g; };
+  const int p_lo = seq.first + row_of(0), p_hi = seq.first + row_of(used - 1);
+  const Visible vis = visible_keys(p, p_lo, p_hi);
   const int chunk = ((vis.count + splits - 1) / splits + 15) / 16 * 16;
   const int v0 = min(vis.count, split * chunk), v1 = min(vis.count, v0 + chunk);
   const int groups = (v1 - v0 + 15) / 16;
@@ -142,18 +156,22 @@ __global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const 
     cp_async_commit();
   }
 
-  // Query fragments: tile rows gq and gq + 8 are heads head0 + gq and head0 + gq + 8.
+  // Query fragments and positions of the tile rows gq and gq + 8.
   uint32_t qa[D / 16][4];
-  {
-    const E *q = static_cast<const E *>(p.q) + seq.start * p.q_stride + (long long)head0 * D;
+  int pos[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = min(gq + 8 * half, used - 1);
+    const bool there = gq + 8 * half < used;
+    pos[half] = seq.first + row_of(r);
+    const E *q = static_cast<const E *>(p.q) + (seq.start + row_of(r)) * p.q_stride + (long long)head_of(r) * D;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = gq + 8 * (i & 1), c = kk * 16 + 2 * tq + 8 * (i >> 1);
-        qa[kk][i] = r < heads ? *reinterpret_cast<const uint32_t *>(q + (long long)r * D + c) : 0u;
-      }
+      for (int i = 0; i < 2; ++i)
+        qa[kk][half + 2 * i] = there ? *reinterpret_cast<const uint32_t *>(q + kk * 16 + 2 * tq + 8 * i) : 0u;
   }
+  bool poisoned = false;  // an infinity or NaN beside masked pairs
   const float scale = p.scale * kLog2e;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
   float acc[D / 8][4];
@@ -190,6 +208,23 @@ __global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const 
           const int key = nt * 8 + 2 * tq + (j & 1);
           if (key >= left || ((bad >> key) & 1)) sc[nt][j] = -INFINITY;
         }
+    }
+    if (ROWS) {
+      const int v = v1 - left, j0 = vis.key(v), j1 = vis.key(v + min(left, 16) - 1);
+      if (j1 > p_lo || (j0 <= p_hi - p.window && j1 >= p.sinks)) {  // not every row sees every key
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = vis.key(v + nt * 8 + 2 * tq + (j & 1)), at = pos[j >> 1];
+            if (k > at || (at - k >= p.window && k >= p.sinks)) sc[nt][j] = -INFINITY;
+          }
+#pragma unroll
+        for (int e = 0; e < kLoads; ++e)
+          poisoned |= any_special(*reinterpret_cast<const uint4 *>(ring + (i % S) * 2 * C::kStageBytes +
+                                                                   C::kStageBytes + (lane + 32 * e) * 16),
+                                  exponent_mask(E()));
+      }
     }
     float rescale[2];
 #pragma unroll
@@ -245,43 +280,56 @@ __global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const 
   }
   pdl_launch_dependents();
   cp_async_wait<0>();
-  __syncthreads();
 
   // Join the warps: their states in shared memory, over the rings.
   float *w_acc = reinterpret_cast<float *>(smem);                                  // [warp][16][D]
   float2 *w_ml = reinterpret_cast<float2 *>(smem + C::kWarps * 16 * D * 4);        // [warp][16]
+  if (ROWS && __syncthreads_or(poisoned)) {  // the rows again, by plain loops; one state each
+    for (int r = warp; r < used; r += C::kWarps) {
+      float mm, ll, o[(D + 31) / 32];
+      slow_row<E, D>(p, seq, s, h, head_of(r), row_of(r), vis, v0, v1, mm, ll, o, lane);
+      for (int w = 0; w < C::kWarps; ++w) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = gq + 8 * half;
-    if (r >= heads) break;
+        for (int n = 0; n < (D + 31) / 32; ++n)
+          if (lane + 32 * n < D) w_acc[(w * 16 + r) * D + lane + 32 * n] = w == 0 ? o[n] : 0.0f;
+        if (lane == 0) w_ml[w * 16 + r] = w == 0 ? make_float2(mm, ll) : make_float2(-INFINITY, 0.0f);
+      }
+    }
+  } else {
+    if (!ROWS) __syncthreads();
 #pragma unroll
-    for (int dt = 0; dt < D / 8; ++dt)
-      *reinterpret_cast<float2 *>(w_acc + (warp * 16 + r) * D + dt * 8 + 2 * tq) =
-          make_float2(acc[dt][2 * half], acc[dt][2 * half + 1]);
-    if (tq == 0) w_ml[warp * 16 + r] = make_float2(m_run[half], l_run[half]);
+    for (int half = 0; half < 2; ++half) {
+      const int r = gq + 8 * half;
+      if (r >= used) break;
+#pragma unroll
+      for (int dt = 0; dt < D / 8; ++dt)
+        *reinterpret_cast<float2 *>(w_acc + (warp * 16 + r) * D + dt * 8 + 2 * tq) =
+            make_float2(acc[dt][2 * half], acc[dt][2 * half + 1]);
+      if (tq == 0) w_ml[warp * 16 + r] = make_float2(m_run[half], l_run[half]);
+    }
   }
   __syncthreads();
   // Join the warps' states, then the CTAs': CTA c of the cluster owns the
-  // elements [c share, (c + 1) share) of the heads x D results; every CTA
+  // elements [c share, (c + 1) share) of the tile's results; every CTA
   // stores its part of them, and its (m, l), in the owner's shared memory, and
   // after one barrier each owner joins what it was sent.
   const int crank = split % cluster, outer = split / cluster, outers = splits / cluster;
-  const int share = ((heads * D + cluster - 1) / cluster + 3) & ~3;
+  const int share = ((used * D + cluster - 1) / cluster + 3) & ~3;
   const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-  const long long slot0 = (long long)s * p.max_rows * p.hq + head0;
   auto finish = [&](int i, const float4 &o, float m, float l) {  // elements i .. i + 3, of one row
+    const int row = row_of(i / D), head = head_of(i / D);
     if (outers > 1) {
-      const int r = i / D;
-      *reinterpret_cast<float4 *>(partial_acc(p, slots, outer, slot0 + r) + i % D) = o;
-      if (i % D == 0) *partial_ml(p, slots, outers, outer, slot0 + r) = make_float2(m, l);
+      const long long slot = ((long long)s * p.max_rows + row) * p.hq + head;
+      *reinterpret_cast<float4 *>(partial_acc(p, slots, outer, slot) + i % D) = o;
+      if (i % D == 0) *partial_ml(p, slots, outers, outer, slot) = make_float2(m, l);
     } else {
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
-      *reinterpret_cast<uint2 *>(static_cast<E *>(p.out) + seq.start * p.out_stride + (long long)head0 * D + i) =
-          make_uint2(pack2(o.x * inv, o.y * inv, E()), pack2(o.z * inv, o.w * inv, E()));
+      *reinterpret_cast<uint2 *>(static_cast<E *>(p.out) + (seq.start + row) * p.out_stride + (long long)head * D +
+                                 i % D) = make_uint2(pack2(o.x * inv, o.y * inv, E()), pack2(o.z * inv, o.w * inv, E()));
     }
   };
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
-  for (int i = tid * 4; i < heads * D; i += 128 * 4) {
+  for (int i = tid * 4; i < used * D; i += 128 * 4) {
     const int r = i / D;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -301,7 +349,7 @@ __global__ void __launch_bounds__(128, kDecodePerSm) window_decode_kernel(const 
   }
   if (cluster == 1) return;
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const int e0 = crank * share, e1 = min(heads * D, e0 + share);
+  const int e0 = crank * share, e1 = min(used * D, e0 + share);
   for (int i = e0 + tid * 4; i < e1; i += 128 * 4) {
     const int r = i / D;
     float m = -INFINITY, l = 0.0f;
@@ -618,7 +666,7 @@ __global__ void __launch_bounds__(kJoinThreads) window_join_kernel(const WindowA
 
 struct Plan {
   bool decode, tensor;
-  int tiles;    // per (sequence, KV head): head tiles (decode), row tiles, or pairs of them (tensor)
+  int tiles;    // per (sequence, KV head): of 16 (row, head) pairs (decode), of 128, or pairs of those (tensor)
   int cluster;  // decode: CTAs that join in distributed shared memory
   int outer;    // splits that join through the workspace
 };
@@ -630,9 +678,12 @@ size_t partial_bytes(int sequences, int max_rows, int hq, int d, int outer) {
 // keys: the most keys a row can see.
 Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long keys, int num_sms) {
   const int g = hq / hkv;
-  Plan plan{max_rows == 1, max_rows > 1 && (d == 64 || d == 128), 1, 1, 1};
-  const long long height = plan.tensor ? 256 : 128;  // tile rows of a prompt CTA
-  plan.tiles = plan.decode ? (g + 15) / 16 : (int)((max_rows * (long long)g + height - 1) / height);
+  const long long tile_rows = (long long)max_rows * g, few_tiles = (tile_rows + 15) / 16 * hkv;  // tiles of decoding
+  const bool few = max_rows == 1 || (few_tiles <= 65535 && (tile_rows <= 16 || (double)few_tiles * sequences * keys * d <=
+                                                                                   kFewElements));
+  Plan plan{few, !few && (d == 64 || d == 128), 1, 1, 1};
+  const long long height = plan.decode ? 16 : plan.tensor ? 256 : 128;  // tile rows of a CTA
+  plan.tiles = (int)((tile_rows + height - 1) / height);
   const long long ctas = (long long)sequences * hkv * plan.tiles;
   const long long slots = (plan.decode ? kDecodePerSm : plan.tensor ? 1 : 2) * num_sms;  // CTAs that run at the same time
   // Tensor-core prompts: one round of CTAs, down to one step of 128 keys each
@@ -723,12 +774,12 @@ cudaError_t launch(const WindowAttentionParams &p, int num_sms, cudaStream_t str
   };
   cudaError_t e;
   if (plan.decode) {
-    const auto kernel = window_decode_kernel<E, D>;
+    const auto kernel = p.max_rows == 1 ? window_decode_kernel<E, D, false> : window_decode_kernel<E, D, true>;
     if ((e = allow_smem(reinterpret_cast<const void *>(kernel), C::smem(16))) != cudaSuccess) return e;
-    const int g = p.hq / p.hkv;
+    const long long rows = (long long)p.max_rows * (p.hq / p.hkv);
     cfg.gridDim = dim3(plan.cluster * plan.outer, p.hkv * plan.tiles, p.sequences);
     cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = C::smem(g < 16 ? g : 16);
+    cfg.dynamicSmemBytes = C::smem(rows < 16 ? (int)rows : 16);
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = plan.cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;

@@ -297,7 +297,7 @@ int tmc_k_paged_attention_f16_noalloc(const void *q, void *out, const void *k_po
  *            positions first_positions[s], first_positions[s] + 1, ..
  *            (below capacity); rows of no sequence are left as they were
  *   rows     rows of q and out; max_rows: the most rows of one sequence (1:
- *            single-token decoding)
+ *            single-token decoding). A close bound: the launch is laid out for it
  * hq a multiple of hkv, d in {16, 32, 64, 128}, scale 0 for 1 / sqrt(d);
  * pointers 16-byte aligned. A row all of whose pages are missing becomes 0.
  * workspace: with tmc_k_window_attention_workspace_bytes(...) bytes a launch of
