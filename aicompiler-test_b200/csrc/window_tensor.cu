@@ -51,12 +51,12 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kKeys = 128;  // of a step
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 3;  // with boxes: one for K, one for V
+constexpr int kLoadWarps = 2;  // with boxes: one for K, one for V
 constexpr int kBox = 16;       // positions of a box
-constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
-constexpr int kFlagRing = 4;  // steps whose missing-key flags are kept: more than the stages
-constexpr float kMostWeight = 8192.0f;  // of a row in one step; fp16 ends at 65504
+constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;  // and the next: one for each tile's products
+constexpr int kThreads = (kMmaWarp + 2) * 32;
+constexpr int kFlagRing = 8;  // steps whose missing-key flags are kept
+constexpr float kSlack = 8.0f;  // powers of two by which the maximum may pass m
 constexpr uint32_t kTmemColumns = 512;
 
 template <int D>
@@ -65,7 +65,7 @@ struct TensorCfg {
   static constexpr int kTile = D / 64 * kHalf;          // one of K, V or a Q tile
   static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kSmem = 1024 + 2 * kTile + kStages * 2 * kTile;
-  static_assert(kStages < kFlagRing, "flags outlive their stage");
+  static_assert(kStages + 1 < kFlagRing, "keys load a stage ahead of the products, those a step ahead of the softmax");
 };
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -147,18 +147,20 @@ __device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_n_major)
   return (1u << 4) | (type << 7) | (type << 10) | ((b_n_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kTileRows >> 4) << 24);
 }
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// One thread (`lead`) issues; the whole warp runs these, so that descriptors
+// stay in uniform registers.
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, bool lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u), "r"(lead ? 1u : 0u)
       : "memory");
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, bool lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u), "r"(lead ? 1u : 0u)
       : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t *bar) {
@@ -203,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char *sQ = base, *sK = base + 2 * C::kTile, *sV = sK + S * C::kTile;
-  __shared__ __align__(8) uint64_t q_full, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2], o_full[2], drained, v_landed;
+  __shared__ __align__(8) uint64_t q_full, k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], s_free[2],
+      p_full[2], p_done[2], o_full[2], drained[2], v_landed;
   __shared__ uint32_t tmem_base;
   __shared__ __align__(16) unsigned char bad_keys[kFlagRing][kKeys];  // keys of a step whose page is missing
   __shared__ int bad_any[kFlagRing][2];
@@ -263,18 +266,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) {
     if (lane == 0) {
       mbar_init(&q_full, kSoftmaxWarps);
-      mbar_init(&drained, 1);
       mbar_init(&v_landed, 1);
       for (int i = 0; i < S; ++i) {
         mbar_init(&k_full[i], BOXES ? 1 : 2);
         mbar_init(&v_full[i], BOXES ? 1 : 2);
-        mbar_init(&k_empty[i], 1);
-        mbar_init(&v_empty[i], 1);
+        mbar_init(&k_empty[i], tiles);
+        mbar_init(&v_empty[i], tiles);
       }
       for (int t = 0; t < 2; ++t) {
         mbar_init(&s_full[t], 1);
+        mbar_init(&s_free[t], 4);
         mbar_init(&p_full[t], 4);
+        mbar_init(&p_done[t], 1);
         mbar_init(&o_full[t], 1);
+        mbar_init(&drained[t], 1);
         marked[t] = 0;
       }
       fence_barrier_init();
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t0 = min(m0 + t * kTileRows, total - 1), t1 = min(m0 + (t + 1) * kTileRows, total) - 1;
     const int p_lo = seq.first + t0 / g, p_hi = seq.first + t1 / g;  // of the tile's rows
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + t * kKeys, o_at = tmem + lanes + 2 * kKeys + t * D;
+    const uint32_t s_at = tmem + lanes, p_at = s_at + kKeys + t * (kKeys / 2), o_at = s_at + 2 * kKeys + t * D;
     const float scale = p.scale * kLog2e;
     float m_run = -INFINITY;
     float2 l_run[2] = {};
@@ -362,60 +367,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const bool missing = (bad_any[j % kFlagRing][0] | bad_any[j % kFlagRing][1]) != 0;
         const bool masked = !whole || missing;
-        auto load = [&](float (&x)[kKeys]) {
-          tmem_load128(s_at, x);
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int v = first + c * 32;
-              uint32_t bits = bits_between(0 - v, min(always, v1) - v) | bits_between(from - v, to - v);
-              if (missing)
-                for (int i = 0; i < 32; ++i)
-                  if (bad_keys[j % kFlagRing][c * 32 + i]) bits &= ~(1u << i);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[c * 32 + i] = (bits >> i) & 1 ? x[c * 32 + i] : -INFINITY;
-            }
-          }
-        };
         float x[kKeys];
-        uint32_t w[kKeys / 2];  // P, two weights to a register
-        float2 sum[2];
-        auto weigh = [&] {
-          // A masked score (-inf) has weight 0; a row that has seen nothing yet has m = -inf.
-          const float about = m_run == -INFINITY ? 0.0f : -m_run;
-          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+        tmem_load128(s_at, x);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);  // the next step's scores may come
+        if (masked) {
 #pragma unroll
-          for (int i = 0; i < kKeys / 2; ++i) {
-            const float2 y = __ffma2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(scale, scale),
-                                        make_float2(about, about));
-            const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-            sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-            w[i] = pack2(e.x, e.y, E());
+          for (int c = 0; c < 4; ++c) {
+            const int v = first + c * 32;
+            uint32_t bits = bits_between(0 - v, min(always, v1) - v) | bits_between(from - v, to - v);
+            if (missing)
+              for (int i = 0; i < 32; ++i)
+                if (bad_keys[j % kFlagRing][c * 32 + i]) bits &= ~(1u << i);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[c * 32 + i] = (bits >> i) & 1 ? x[c * 32 + i] : -INFINITY;
           }
-          return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        };
-        // Weights about the present m; where they are too large, m moves and the
-        // step is weighed again. The first step starts with its maximum.
-        load(x);
-        bool rise = true;
-#pragma unroll 1
-        for (int round = j == 0 ? 1 : 0;; ++round) {
-          if (round != 1) {
-            const float total_weight = weigh();
-            if (round > 1) break;
-            rise = total_weight > kMostWeight || m_run == -INFINITY;
-            if (!__any_sync(0xffffffffu, rise)) break;
-            load(x);
-            continue;
-          }
-          float y[8];
+        }
+        float y[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i];
+        for (int i = 0; i < 8; ++i) y[i] = x[i];
 #pragma unroll
-          for (int i = 8; i < kKeys; ++i) y[i % 8] = fmaxf(y[i % 8], x[i]);
-          const float mx = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
-                                 fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))) * scale;
-          rise = rise && mx > m_run;
+        for (int i = 8; i < kKeys; i += 16)
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            y[n] = i + 8 + n < kKeys ? fmaxf(fmaxf(y[n], x[i + n]), x[i + 8 + n]) : fmaxf(y[n], x[i + n]);
+        const float mx =
+            fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))) * scale;
+        const bool rise = mx > m_run + kSlack || (m_run == -INFINITY && mx > m_run);
+        // The products of the step before: O is complete, P's place free.
+        if (j > 0 && !__all_sync(0xffffffffu, wait(&p_done[t], (j - 1) & 1))) {
+          if (lane == 0) gave_up(j);
+          failed = true;
+          break;
+        }
+        if (__any_sync(0xffffffffu, rise)) {
           const float f = rise ? exp2_fast(m_run - mx) : 1.0f;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -423,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             l_run[i].y *= f;
           }
           if (rise) m_run = mx;
-          if (j > 0) {  // S of this step was issued after O's last product: O is complete
+          if (j > 0) {
+            fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               float o[16];
@@ -433,11 +420,21 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 16; ++i) scaled[i] = __float_as_uint(o[i] * f);
               tmem_store16(o_at + c, scaled);
             }
+            wait_st();
           }
         }
+        // A masked score (-inf) has weight 0; a row that has seen nothing yet has m = -inf.
+        const float about = m_run == -INFINITY ? 0.0f : -m_run;
+        uint32_t w[kKeys / 2];  // P, two weights to a register
 #pragma unroll
-        for (int i = 0; i < 2; ++i) l_run[i] = __fadd2_rn(l_run[i], sum[i]);
-        tmem_store64(s_at, w);  // over S, which has been read
+        for (int i = 0; i < kKeys / 2; ++i) {
+          const float2 z = __ffma2_rn(make_float2(x[2 * i], x[2 * i + 1]), make_float2(scale, scale),
+                                      make_float2(about, about));
+          const float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+          l_run[i & 1] = __fadd2_rn(l_run[i & 1], e);
+          w[i] = pack2(e.x, e.y, E());
+        }
+        tmem_store64(p_at, w);
         wait_st();
         fence_before();
         __syncwarp();
@@ -629,52 +626,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[st]);
     }
-  } else if (lane == 0) {
+  } else {
     // ---- products ----
     constexpr uint32_t kScores = instruction<E>(kKeys, false), kOutputs = instruction<E>(D, true);
-    bool ok = mbar_wait(&q_full, 0);
-    auto scores = [&](int t, int j) {
-      const uint32_t q = smem_u32(sQ + t * C::kTile), k = smem_u32(sK + (j % S) * C::kTile);
+    const bool lead = lane == 0;
+    const int t = warp - kMmaWarp;
+    const uint64_t q = k_major(smem_u32(sQ + t * C::kTile)), k_at = k_major(smem_u32(sK)),
+                   v_at = n_major(smem_u32(sV), C::kHalf);
+    const uint32_t o = tmem + 2 * kKeys + t * D, weights = tmem + kKeys + t * (kKeys / 2);
+    auto here = [&](uint64_t *bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase & 1)); };
+    auto arrive = [&](uint64_t *bar) {  // when the products so far are done
+      if (lead) commit(bar);
+      __syncwarp();
+    };
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&q_full, 0));
+    // S = Q K^T of step j, once the scores that were there have been read: the
+    // tiles take turns.
+    auto scores = [&](int j) {
+      ok = ok && here(&k_full[j % S], j / S);
+      if (tiles == 1 ? j > 0 : t == 1 || j > 0) ok = ok && here(&s_free[tiles == 1 ? 0 : 1 - t], t == 1 ? j : j - 1);
+      if (!ok) return;
+      fence_after();
+      const uint64_t k = k_at + (j % S) * (C::kTile >> 4);
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        const uint32_t off = (i / 4) * C::kHalf + (i % 4) * 32;
-        mma_smem(tmem + t * kKeys, k_major(q + off), k_major(k + off), kScores, i > 0);
+        const int off = (i / 4) * (C::kHalf >> 4) + (i % 4) * (32 >> 4);
+        mma_smem(tmem, q + off, k + off, kScores, i > 0, lead);
       }
-      commit(&s_full[t]);
+      arrive(&s_full[t]);
+      arrive(&k_empty[j % S]);
     };
-    ok = ok && wait(&k_full[0], 0);
-    fence_after();
-    if (ok) {
-      for (int t = 0; t < tiles; ++t) scores(t, 0);
-      commit(&k_empty[0]);
-    }
-    for (int j = 0; j < steps && ok; ++j) {
-      const int st = j % S;
-      ok = wait(&v_full[st], (j / S) & 1);
-      if (j + 1 < steps) ok = ok && wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1);
-      for (int t = 0; t < tiles && ok; ++t) {
-        ok = wait(&p_full[t], j & 1);
-        if (!ok) break;
-        fence_after();
-        const uint32_t v = smem_u32(sV + st * C::kTile);
-#pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
-          mma_tmem(tmem + 2 * kKeys + t * D, tmem + t * kKeys + i * 8, n_major(v + i * 16 * 128, C::kHalf), kOutputs,
-                   j > 0 || i > 0);
-        if (j + 1 < steps)
-          scores(t, j + 1);
-        else
-          commit(&o_full[t]);
-      }
+    if (t < tiles) scores(0);
+    for (int j = 0; t < tiles && j < steps && ok; ++j) {
+      if (j + 1 < steps) scores(j + 1);
+      // O += P V of step j.
+      ok = ok && here(&v_full[j % S], j / S) && here(&p_full[t], j);
       if (!ok) break;
-      commit(&v_empty[st]);
-      if (j + 1 < steps) commit(&k_empty[(j + 1) % S]);
+      fence_after();
+      const uint64_t v = v_at + (j % S) * (C::kTile >> 4);
+#pragma unroll
+      for (int i = 0; i < kKeys / 16; ++i)
+        mma_tmem(o, weights + i * 8, v + i * (16 * 128 >> 4), kOutputs, j > 0 || i > 0, lead);
+      arrive(&p_done[t]);
+      if (j + 1 == steps) arrive(&o_full[t]);
+      arrive(&v_empty[j % S]);
     }
     if (!ok) {
       // Something never came: the products in flight end (a bounded wait) before the memory is given back.
-      gave_up(-1);
-      commit(&drained);
-      (void)mbar_wait(&drained, 0);
+      if (lead) gave_up(-1);
+      arrive(&drained[t]);
+      (void)mbar_wait(&drained[t], 0);
     }
   }
   pdl_launch_dependents();
