@@ -2,19 +2,22 @@
 // and 128; see window_attention.cu for the other shapes and for decoding).
 //
 // A CTA holds two tiles of 128 tile rows (query row x head of one KV head) and
-// walks the visible keys 128 at a time: S_t = Q_t K^T and O_t += P_t V by
-// tcgen05.mma, S, P and O in tensor memory (P, in the storage type, over the
-// first half of its S). Four warps per tile are its softmax, one thread per
-// tile row: while one tile's exponentials are taken the other tile's products
-// run. K and V come in through the block table: pages of whole groups of 16
-// positions as TMA boxes (the key numbering starts on a group then, and what
-// no row sees of a group is zeroed in V), other page sizes as 16-byte copies
-// by three warps. One thread issues the products.
+// walks the visible keys 128 at a time: S = Q_t K^T and O_t += P_t V by
+// tcgen05.mma, S, P and O in tensor memory. The tiles take turns in one S (128
+// columns): a tile's softmax reads it whole into registers, and the other's
+// scores are computed while it takes its exponentials, so that each finds its
+// next scores waiting. P (the storage type, 64 columns) and O have places of
+// their own. Four warps per tile are its softmax, one thread per tile row; one
+// warp per tile issues its products, so that the waits of one pass under the
+// products of the other. K and V come in through the block table by two warps:
+// pages of whole groups of 16 or 8 positions as TMA boxes (the key numbering
+// starts on a group then, and what no row sees of a group is zeroed in V), other
+// page sizes as 16-byte copies.
 //
-// Weights are 2^(s - m) about a number m per row that only moves, to the
-// maximum seen, when a step's weights sum to more than kMostWeight: sums in
-// fp32 and P's floating-point numbers lose nothing below that, and neither the
-// maximum is taken nor O rescaled in most steps.
+// Weights are 2^(s - m) about a number m per row that moves to the maximum only
+// when that has passed it by more than kSlack: sums in fp32 and P's
+// floating-point numbers lose nothing below that, and O is not rescaled in most
+// steps.
 //
 // P is rounded once to the storage type; the row sum l is taken before that.
 // Each output then carries independent errors of half a step per key, which
@@ -24,19 +27,20 @@
 // would reach that row as 0 x inf: such a step marks the tile, and the tile's
 // rows are computed again by plain loops.
 //
-// Bound: per 128 keys a tile's softmax takes 2140 cycles and its products 1330,
-// of which two tiles overlap most: 8192 rows x 32 heads of 128 causally 580 us,
-// 948 TFLOP/s, 0.57 of a library product's short-run rate and 0.69 of its rate
-// under the power limit (the products alone 418 us of 605 in an earlier version,
-// the softmax alone 459). Measured and left out: two
-// threads a row (656 us against 620), P handed over in halves (614 against
-// 606), an eighth to a half of the exponentials as polynomials (636 to 651
-// against 598), steps of 64 keys with S double-buffered (820 against 606: a
-// product with N = 64 takes as long as with 128), the splits joined in clusters
-// (512 rows over 8k keys 84 us against 88, but 57 against 33 where clusters of
-// six leave SMs idle). Short calls are set-up and hand-over: 256 rows x 32
-// heads, window 512, 21 us, of which reading the first keys 4, a step 2, the
-// results 2 to 3 and the joining kernel 4.
+// Bound: the tensor pipe, at 81 to 90 cycles per product of 128 x 128 x 16 (a
+// library product runs at 88), 32 of them per 128 keys of both tiles, beside a
+// softmax of 2200 to 2700 cycles: 8192 rows x 32 heads of 128 causally 533 us,
+// 1032 TFLOP/s, 0.62 of the library product's short-run rate and 0.75 of its
+// rate under the power limit. With P over its own S, scores waited for the
+// products before them (592 us); one warp for both tiles' products (606); P in
+// shared memory (644: both operands from there). Before that, measured and left
+// out: two threads a row, P handed over in halves, an eighth to a half of the
+// exponentials as polynomials, steps of 64 keys (a product with N = 64 takes as
+// long as with 128), the splits joined in clusters (512 rows over 8k keys 84 us
+// against 88, but 57 against 33 where clusters of six leave SMs idle). Short
+// calls are set-up and hand-over: 256 rows x 32 heads, window 512, 21 us, of
+// which reading the first keys 4, a step 2, the results 2 to 3 and the joining
+// kernel 4.
 #include <map>
 #include <mutex>
 #include <utility>
@@ -51,8 +55,7 @@ namespace {
 constexpr int kTileRows = 128;
 constexpr int kKeys = 128;  // of a step
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 2;  // with boxes: one for K, one for V
-constexpr int kBox = 16;       // positions of a box
+constexpr int kLoadWarps = 2;  // with boxes one for K, one for V
 constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;  // and the next: one for each tile's products
 constexpr int kThreads = (kMmaWarp + 2) * 32;
 constexpr int kFlagRing = 8;  // steps whose missing-key flags are kept
@@ -183,6 +186,15 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
       : "memory");
   return done || mbar_wait(bar, parity);
 }
+__device__ __forceinline__ bool through(uint64_t *bar, uint32_t parity) {  // at this moment
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
 // Bits [a, b) of 32.
 __device__ __forceinline__ uint32_t bits_between(int a, int b) {
   a = max(a, 0);
@@ -195,11 +207,14 @@ __device__ __forceinline__ int swizzled(int r, int c) {
   return (c >> 3) * (kKeys * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// Grid as prompt_place counts it, over tile pairs. BOXES: K and V by TMA boxes.
-template <typename E, int D, bool BOXES>
+// Grid as prompt_place counts it, over tile pairs. BOX: positions of the TMA
+// boxes that bring K and V, 0 without.
+template <typename E, int D, int BOX>
 __global__ void __launch_bounds__(kThreads, 1)
     window_tensor_kernel(const WindowAttentionParams p, int splits, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map) {
+  constexpr bool BOXES = BOX > 0;
+  constexpr int kBox = BOXES ? BOX : 16;
   using C = TensorCfg<D>;
   constexpr int S = C::kStages;
   extern __shared__ unsigned char smem_raw[];
@@ -585,6 +600,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // to the warps in the order in which they are needed ----
     const int load = warp - kSoftmaxWarps;
     KeyPlace next[2] = {first_half[0], first_half[1]};
+    uint64_t *late = nullptr;  // of the job whose copies may be in flight beside this one's
+    auto landed = [&] {
+      fence_async();  // what the copies wrote, before the products read it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(late);
+    };
     for (int job = load; job < 4 * steps; job += kLoadWarps) {
       const int j = job >> 2, st = j % S, half = job & 1;
       const bool value = (job & 2) != 0;
@@ -598,9 +619,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         next[i] = find_half(job + kLoadWarps, i);
       }
       uint64_t *full = value ? v_full : k_full, *empty = value ? v_empty : k_empty;
-      if (j >= S && !__all_sync(0xffffffffu, wait(&empty[st], ((j / S) - 1) & 1))) {
-        if (lane == 0) gave_up(j);
-        break;
+      if (j >= S) {
+        const uint32_t phase = ((j / S) - 1) & 1;
+        if (late && !__all_sync(0xffffffffu, through(&empty[st], phase))) {  // its place may wait for those copies
+          cp_async_wait<0>();
+          landed();
+          late = nullptr;
+        }
+        if (!__all_sync(0xffffffffu, wait(&empty[st], phase))) {
+          if (lane == 0) gave_up(j);
+          break;
+        }
       }
       if (!value) {
         bad_keys[j % kFlagRing][half * 64 + lane] = bad[0];
@@ -621,10 +650,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           cp_async16(dst + swizzled(i * 32 + r, c), pool + (size_t)(there ? row : 0u) * (D * 2), there ? 16 : 0);
         }
       cp_async_commit();
+      if (late) {
+        cp_async_wait<1>();
+        landed();
+      }
+      late = &full[st];
+    }
+    if (late) {
       cp_async_wait<0>();
-      fence_async();  // what the copies wrote, before the products read it
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st]);
+      landed();
     }
   } else {
     // ---- products ----
@@ -688,14 +722,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <typename E, int D, bool BOXES>
+template <typename E, int D, int BOX>
 cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaStream_t stream, bool pdl) {
-  const auto kernel = window_tensor_kernel<E, D, BOXES>;
+  const auto kernel = window_tensor_kernel<E, D, BOX>;
   CUtensorMap k_map{}, v_map{};
-  if (BOXES) {  // 16-bit elements of either kind: boxes only move them
+  if (BOX > 0) {  // 16-bit elements of either kind: boxes only move them
     const uint64_t rows = (uint64_t)p.pool_pages * p.hkv * p.page_size;
-    cudaError_t e = make_tensor_map_f16(&k_map, p.k_pool, rows, D, kBox);
-    if (e == cudaSuccess) e = make_tensor_map_f16(&v_map, p.v_pool, rows, D, kBox);
+    cudaError_t e = make_tensor_map_f16(&k_map, p.k_pool, rows, D, BOX);
+    if (e == cudaSuccess) e = make_tensor_map_f16(&v_map, p.v_pool, rows, D, BOX);
     if (e != cudaSuccess) return e;
   }
   {
@@ -724,22 +758,29 @@ cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaSt
   return cudaLaunchKernelEx(&cfg, kernel, p, splits, k_map, v_map);
 }
 
-template <typename E>
+template <typename E, int D>
 cudaError_t dispatch(const WindowAttentionParams &p, int pairs, int splits, cudaStream_t stream, bool pdl) {
-  const bool boxes = p.page_size % kBox == 0 && (long long)p.pool_pages * p.hkv <= 0x7fffffffll / p.page_size;
-  if (p.d == 64)
-    return boxes ? launch<E, 64, true>(p, pairs, splits, stream, pdl) : launch<E, 64, false>(p, pairs, splits, stream, pdl);
-  if (p.d == 128)
-    return boxes ? launch<E, 128, true>(p, pairs, splits, stream, pdl)
-                 : launch<E, 128, false>(p, pairs, splits, stream, pdl);
-  return cudaErrorInvalidValue;
+  // Boxes of 16 positions where pages are whole numbers of them, else of 8 (4096
+  // rows, pages of 24: 165 us, by copies 209; pages of 16: 158, by boxes of 16
+  // 144). Pool rows are 32-bit coordinates.
+  if ((long long)p.pool_pages * p.hkv <= 0x7fffffffll / p.page_size) {
+    if (p.page_size % 16 == 0) return launch<E, D, 16>(p, pairs, splits, stream, pdl);
+    if (p.page_size % 8 == 0) return launch<E, D, 8>(p, pairs, splits, stream, pdl);
+  }
+  return launch<E, D, 0>(p, pairs, splits, stream, pdl);
 }
 
 }  // namespace
 
 cudaError_t launch_window_tensor(const WindowAttentionParams &p, bool bf16, int pairs, int splits, cudaStream_t stream,
                                  bool pdl) {
-  return bf16 ? dispatch<__nv_bfloat16>(p, pairs, splits, stream, pdl) : dispatch<__half>(p, pairs, splits, stream, pdl);
+  using Bf16 = __nv_bfloat16;
+  if (p.d == 64)
+    return bf16 ? dispatch<Bf16, 64>(p, pairs, splits, stream, pdl) : dispatch<__half, 64>(p, pairs, splits, stream, pdl);
+  if (p.d == 128)
+    return bf16 ? dispatch<Bf16, 128>(p, pairs, splits, stream, pdl)
+                : dispatch<__half, 128>(p, pairs, splits, stream, pdl);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace window
