@@ -410,13 +410,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mx =
             fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7]))) * scale;
         const bool rise = mx > m_run + kSlack || (m_run == -INFINITY && mx > m_run);
-        // The products of the step before: O is complete, P's place free.
-        if (j > 0 && !__all_sync(0xffffffffu, wait(&p_done[t], (j - 1) & 1))) {
-          if (lane == 0) gave_up(j);
-          failed = true;
-          break;
-        }
+        // After the products of the step before, O is complete and P's place free.
+        auto products_done = [&] { return j == 0 || __all_sync(0xffffffffu, wait(&p_done[t], (j - 1) & 1)); };
         if (__any_sync(0xffffffffu, rise)) {
+          if (!products_done()) {
+            if (lane == 0) gave_up(j);
+            failed = true;
+            break;
+          }
           const float f = rise ? exp2_fast(m_run - mx) : 1.0f;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -449,6 +450,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           l_run[i & 1] = __fadd2_rn(l_run[i & 1], e);
           w[i] = pack2(e.x, e.y, E());
         }
+        if (!products_done()) {
+          if (lane == 0) gave_up(j);
+          failed = true;
+          break;
+        }
+        fence_after();
         tmem_store64(p_at, w);
         wait_st();
         fence_before();
