@@ -43,8 +43,8 @@ constexpr int kMaxOuter = 32;  // splits that meet through the workspace
 // Prompts of at most 16 tile rows, or so short that all of their 16-row tiles
 // together read no more than this (elements of keys), run as decoding does: it
 // has less to set up, but reads the keys for every 16 rows. 32 heads, 8 KV heads
-// of 128: 2 rows over 1000 keys 7.7 us (as prompts 13.9), 16 rows 10.8 (14.6), 32
-// rows (8.5 million) 14.9 (15.0), 64 rows (17 million) 20.1 (17.1); 64 sequences
+// of 128: 2 rows over 1000 keys 7.7 us (as prompts 13.9), 16 rows 10.7 (14.5), 32
+// rows (8.2 million) 14.8 (14.7), 64 rows (16 million) 20.0 (17.1); 64 sequences
 // of 4 rows over 1000 to 2000 keys 100 us (131), 16 heads of 64 of their own 92 (211).
 constexpr long long kFewElements = 12500000;
 

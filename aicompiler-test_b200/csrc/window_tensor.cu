@@ -27,13 +27,15 @@
 // would reach that row as 0 x inf: such a step marks the tile, and the tile's
 // rows are computed again by plain loops.
 //
-// Bound: the tensor pipe, at 81 to 90 cycles per product of 128 x 128 x 16 (a
-// library product runs at 88), 32 of them per 128 keys of both tiles, beside a
-// softmax of 2200 to 2700 cycles: 8192 rows x 32 heads of 128 causally 533 us,
-// 1032 TFLOP/s, 0.62 of the library product's short-run rate and 0.75 of its
+// Bound: the tensor pipe, at 81 to 90 cycles per product of 128 x 128 x 16 (88
+// would be 1675 TFLOP/s, a library product's, at 1.9 GHz), 32 of them per 128 keys of both tiles, beside a
+// softmax of 2200 to 2700 cycles: 8192 rows x 32 heads of 128 causally 520 us,
+// 1057 TFLOP/s, 0.63 of the library product's short-run rate and 0.77 of its
 // rate under the power limit. With P over its own S, scores waited for the
 // products before them (592 us); one warp for both tiles' products (606); P in
-// shared memory (644: both operands from there). Before that, measured and left
+// shared memory (644: both operands from there); an S of its own for each tile
+// where heads of 64 leave room (2 x 4096 rows 258 us against 234: the tiles then
+// take their exponentials at the same time). Before that, measured and left
 // out: two threads a row, P handed over in halves, an eighth to a half of the
 // exponentials as polynomials, steps of 64 keys (a product with N = 64 takes as
 // long as with 128), the splits joined in clusters (512 rows over 8k keys 84 us
