@@ -755,9 +755,9 @@ std::string DecoderExecutor::copyPages(const std::vector<KVPageCopy> &copies) {
   return {};
 }
 
-std::string DecoderExecutor::prepareAppend(int slot) {
+std::string DecoderExecutor::prepareAppend(int slot, std::size_t end) {
   std::vector<KVPageCopy> copies;
-  auto e = slots_[slot]->unshareTail(&copies);
+  auto e = slots_[slot]->unshareTail(&copies, end);
   return e.empty() ? copyPages(copies) : e;
 }
 
@@ -1488,7 +1488,7 @@ std::string DecoderExecutor::decode(const std::int32_t *slots, const std::int32_
     auto &st = *slots_[slots[staged]];
     positions[staged] = static_cast<std::int32_t>(st.currentLength());
     tableRows[staged] = slots[staged];
-    err = prepareAppend(slots[staged]);
+    err = prepareAppend(slots[staged], st.currentLength() + 1);
     if (err.empty()) err = st.stageLength(st.currentLength() + 1);
     if (!err.empty()) break;
   }
@@ -1656,7 +1656,7 @@ std::string DecoderExecutor::runPrefill(int slot, const std::int32_t *tokens, in
     if (tokens[i] < 0 || tokens[i] >= cfg_.vocab) return "prefill: token id out of vocabulary range.";
   auto &st = *slots_[slot];
   const size_t start = st.currentLength();
-  auto err = prepareAppend(slot);
+  auto err = prepareAppend(slot, start + count);
   if (err.empty()) err = st.stageLength(start + count);
   if (!err.empty()) return err;
   std::vector<std::int32_t> targets;  // of every position: the token behind it
@@ -1748,7 +1748,7 @@ std::string DecoderExecutor::generate(const std::int32_t *slots, const std::int3
     auto &st = *slots_[slots[staged]];
     positions[staged] = static_cast<std::int32_t>(st.currentLength());
     tableRows[staged] = slots[staged];
-    err = prepareAppend(slots[staged]);
+    err = prepareAppend(slots[staged], st.currentLength() + steps);
     if (err.empty()) err = st.stageLength(st.currentLength() + steps);
     if (!err.empty()) break;
   }

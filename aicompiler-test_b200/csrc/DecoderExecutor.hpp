@@ -223,8 +223,8 @@ class DecoderExecutor {
   std::string ensurePoolPointers();
   std::string ensurePageLists(std::size_t count);
   std::string copyPages(const std::vector<KVPageCopy> &copies);
-  // A slot's next position falls into a page of its own.
-  std::string prepareAppend(int slot);
+  // The slot's positions from its length up to `end` fall into pages of its own.
+  std::string prepareAppend(int slot, std::size_t end);
   std::string ensureScores();
   // Scores of `rows` rows of logits_ into host memory at row `at`, enqueued.
   std::string enqueueScores(const std::int32_t *targets, int rows, const TokenScores &out, std::size_t at);

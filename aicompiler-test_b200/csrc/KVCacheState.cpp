@@ -181,25 +181,37 @@ std::string KVCacheState::fork(const KVCacheState &source, std::vector<KVPageCop
   return {};
 }
 
-std::string KVCacheState::unshareTail(std::vector<KVPageCopy> *copies) {
-  const auto logical = currentLength_ / pool_->pageSize();
-  if (logical >= logicalToPhysical_.size()) return {};
-  const auto shared = logicalToPhysical_[logical];
-  if (pool_->owners(shared) < 2) return {};
-  const auto page = pool_->allocatePage();
-  if (page < 0) return "Paged KV cache physical page pool is exhausted.";
-  logicalToPhysical_[logical] = page;
+std::string KVCacheState::unshareTail(std::vector<KVPageCopy> *copies, std::size_t end) {
+  const auto size = pool_->pageSize();
+  const auto pages = std::min(allocatedPageCount(), end / size + (end % size != 0 ? 1 : 0));
+  auto row = logicalToPhysical_;
+  std::vector<KVPageCopy> taken;
+  const auto giveBack = [&] {
+    for (const auto &t : taken) pool_->releasePage(t.to);
+  };
+  for (auto logical = currentLength_ / size; logical < pages; ++logical) {
+    if (pool_->owners(row[logical]) < 2) continue;
+    const auto page = pool_->allocatePage();
+    if (page < 0) {
+      giveBack();
+      return "Paged KV cache physical page pool is exhausted.";
+    }
+    taken.push_back({row[logical], page});
+    row[logical] = page;
+  }
+  if (taken.empty()) return {};
+  std::swap(row, logicalToPhysical_);
   if (sink_) {
     const auto error = sink_(slot_, logicalToPhysical_);
     if (!error.empty()) {
-      logicalToPhysical_[logical] = shared;
-      pool_->releasePage(page);
+      std::swap(row, logicalToPhysical_);
+      giveBack();
       (void)sink_(slot_, logicalToPhysical_);
       return error;
     }
   }
-  pool_->releasePage(shared);
-  copies->push_back({shared, page});
+  for (const auto &t : taken) pool_->releasePage(t.from);
+  copies->insert(copies->end(), taken.begin(), taken.end());
   return {};
 }
 

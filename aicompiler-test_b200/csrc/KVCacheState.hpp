@@ -19,13 +19,14 @@
 //   * a page may belong to several sequences (forks of one prompt): the pool
 //     counts its owners and frees it with the last one. A sequence writes only
 //     into pages of its own: a fork gets a copy of the partly filled last page,
-//     and a sequence rolled back into a shared page replaces it by a copy
-//     before it appends (unshareTail).
+//     and a sequence whose length was lowered replaces the shared pages that
+//     the next positions fall into by copies before it appends (unshareTail).
 #pragma once
 
 #include <cstddef>
 #include <cstdint>
 #include <functional>
+#include <limits>
 #include <memory>
 #include <string>
 #include <vector>
@@ -107,9 +108,11 @@ class KVCacheState {
   // and take a page for the partly filled one, which the caller then copies
   // (appended to `copies`). All or nothing.
   [[nodiscard]] std::string fork(const KVCacheState &source, std::vector<KVPageCopy> *copies);
-  // Before positions are appended: when the page that the next one falls into
-  // is shared, take one of its own for it, to be copied by the caller.
-  [[nodiscard]] std::string unshareTail(std::vector<KVPageCopy> *copies);
+  // Before the positions [currentLength, end) are appended: take a page of its
+  // own for every shared one that they fall into (a lowered length leaves the
+  // pages behind it in place), to be copied by the caller. All or nothing.
+  [[nodiscard]] std::string unshareTail(std::vector<KVPageCopy> *copies,
+                                        std::size_t end = std::numeric_limits<std::size_t>::max());
   // Keep the first `lead` pages, put `pages` (allocated by the caller) behind
   // them in place of the others and commit `length`. On failure nothing changes.
   [[nodiscard]] std::string replaceTail(std::size_t lead, const std::vector<std::int32_t> &pages, std::size_t length);
