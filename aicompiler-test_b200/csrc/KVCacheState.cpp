@@ -158,6 +158,7 @@ std::string KVCacheState::fork(const KVCacheState &source, std::vector<KVPageCop
   const auto length = source.currentLength_, size = pool_->pageSize();
   if (pool_ != source.pool_ || length == 0 || length > capacity_) return "A fork needs a sequence of the same pool to fork from.";
   const auto full = length / size, pages = (length + size - 1) / size;
+  if (pages > source.allocatedPageCount()) return "A fork needs a page for every committed position.";
   std::int32_t tail = -1;
   if (pages > full) {
     tail = pool_->allocatePage();

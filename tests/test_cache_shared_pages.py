@@ -36,3 +36,16 @@ def test_several_own_pages_are_taken_whole_or_not_at_all(kv):  # noqa: F811
     assert w.pages(1) == before and w.sent(1) == before and w.used() == 4 and [w.owners(p) for p in before] == [2] * 4
     assert len(w.unshare(1)) == 2 and w.used() == 6
     w.close()
+
+
+def test_committed_positions_without_pages_cannot_be_forked(kv):  # noqa: F811
+    w = World(kv)
+    assert kv.kv_state_stage(w.states[0], 4) == 0
+    for length in (10, 5, 16):  # more than the one page that is there
+        assert kv.kv_state_commit(w.states[0], length) == 0
+        assert w.fork(0, 1) == -1 and b"every committed position" in kv.kv_last_error()
+        assert w.used() == 1 and w.pages(1) == [] and kv.kv_state_length(w.states[1]) == 0
+        assert w.owners(w.pages(0)[0]) == 1
+    assert kv.kv_state_commit(w.states[0], 3) == 0
+    assert w.fork(0, 1) == [(w.pages(0)[0], w.pages(1)[0])]
+    w.close()

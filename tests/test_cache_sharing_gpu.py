@@ -34,3 +34,13 @@ def test_appending_behind_a_lowered_length_leaves_the_other_sequence(rt, page_si
             assert np.array_equal(x, y)
         for x, y in zip(m.dec.read_kv(layer, 1), other.read_kv(layer, 1)):
             assert np.array_equal(x, y)
+
+
+def test_committed_positions_without_pages_cannot_be_forked(rt):
+    import tmc_cuda
+    m = Model(rt)
+    m.dec.stage(0, 20)
+    m.dec.commit(0, 100)
+    with pytest.raises(tmc_cuda.TmcError, match="every committed position"):
+        m.dec.fork(0, [1, 2])
+    assert m.dec.pool_stats()["used"] == 2 and m.dec.length(1) == m.dec.length(2) == 0
