@@ -757,8 +757,7 @@ std::string DecoderExecutor::copyPages(const std::vector<KVPageCopy> &copies) {
 
 std::string DecoderExecutor::prepareAppend(int slot, std::size_t end) {
   std::vector<KVPageCopy> copies;
-  auto e = slots_[slot]->unshareTail(&copies, end);
-  return e.empty() ? copyPages(copies) : e;
+  return slots_[slot]->unshareTail(&copies, end, [this](const std::vector<KVPageCopy> &c) { return copyPages(c); });
 }
 
 std::string DecoderExecutor::forkSlot(int slot, const std::int32_t *slots, int count) {

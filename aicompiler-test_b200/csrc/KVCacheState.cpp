@@ -182,7 +182,7 @@ std::string KVCacheState::fork(const KVCacheState &source, std::vector<KVPageCop
   return {};
 }
 
-std::string KVCacheState::unshareTail(std::vector<KVPageCopy> *copies, std::size_t end) {
+std::string KVCacheState::unshareTail(std::vector<KVPageCopy> *copies, std::size_t end, const PageCopier &copy) {
   const auto size = pool_->pageSize();
   const auto pages = std::min(allocatedPageCount(), end / size + (end % size != 0 ? 1 : 0));
   auto row = logicalToPhysical_;
@@ -201,6 +201,13 @@ std::string KVCacheState::unshareTail(std::vector<KVPageCopy> *copies, std::size
     row[logical] = page;
   }
   if (taken.empty()) return {};
+  if (copy) {
+    const auto error = copy(taken);
+    if (!error.empty()) {
+      giveBack();
+      return error;
+    }
+  }
   std::swap(row, logicalToPhysical_);
   if (sink_) {
     const auto error = sink_(slot_, logicalToPhysical_);

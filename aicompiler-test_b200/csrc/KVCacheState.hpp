@@ -77,6 +77,9 @@ struct KVPageCopy {
   std::int32_t to;
 };
 
+// Fills pages; an error text when it could not.
+using PageCopier = std::function<std::string(const std::vector<KVPageCopy> &copies)>;
+
 // Receives a sequence's block-table row whenever its page list changes.
 using BlockTableSink = std::function<std::string(int slot, const std::vector<std::int32_t> &row)>;
 
@@ -110,9 +113,12 @@ class KVCacheState {
   [[nodiscard]] std::string fork(const KVCacheState &source, std::vector<KVPageCopy> *copies);
   // Before the positions [currentLength, end) are appended: take a page of its
   // own for every shared one that they fall into (a lowered length leaves the
-  // pages behind it in place), to be copied by the caller. All or nothing.
+  // pages behind it in place). `copy` fills them before they take the shared
+  // ones' places; without it the caller does, from what `copies` gains. All or
+  // nothing.
   [[nodiscard]] std::string unshareTail(std::vector<KVPageCopy> *copies,
-                                        std::size_t end = std::numeric_limits<std::size_t>::max());
+                                        std::size_t end = std::numeric_limits<std::size_t>::max(),
+                                        const PageCopier &copy = {});
   // Keep the first `lead` pages, put `pages` (allocated by the caller) behind
   // them in place of the others and commit `length`. On failure nothing changes.
   [[nodiscard]] std::string replaceTail(std::size_t lead, const std::vector<std::int32_t> &pages, std::size_t length);
