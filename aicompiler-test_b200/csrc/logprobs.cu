@@ -202,15 +202,21 @@ struct Pass {
     s[i & 1] = __fadd2_rn(s[i & 1], e);
     u[i & 1] = __ffma2_rn(e, d, u[i & 1]);
   }
+  // Before the target come the larger logits behind it and those below it that
+  // reach `reach`: its logit, or NaN (none) for a target at -inf, which all
+  // lower indices come before.
+  static __device__ __forceinline__ bool comes_before(float x, int at, float xt, float reach, int target) {
+    return (at > target && x > xt) || (at < target && x >= reach);
+  }
   // One logit.
-  __device__ __forceinline__ void take(float x, int at, float xt, int target) {
+  __device__ __forceinline__ void take(float x, int at, float xt, float reach, int target) {
     raise(x, at);
     weigh(x, -INFINITY, m == -INFINITY ? 0.0f : m, 0);  // -inf weighs nothing
-    before += (x > xt || (x == xt && at < target)) ? 1.0f : 0.0f;
+    before += comes_before(x, at, xt, reach, target) ? 1.0f : 0.0f;
   }
   // V vectors, `step` vectors apart, the first at index `at`.
   template <int V>
-  __device__ __forceinline__ void take(const uint4 *raw, int at, int step, float xt, int target) {
+  __device__ __forceinline__ void take(const uint4 *raw, int at, int step, float xt, float reach, int target) {
     float mx[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) mx[v] = L::largest(raw[v]);
@@ -230,12 +236,12 @@ struct Pass {
       if (first > target) {
         before += L::template above<false>(raw[v], xt);
       } else if (first + N <= target) {
-        before += L::template above<true>(raw[v], xt);
+        before += L::template above<true>(raw[v], reach);
       } else {
         float x[N];
         L::unpack(raw[v], x);
 #pragma unroll
-        for (int i = 0; i < N; ++i) before += (x[i] > xt || (x[i] == xt && first + i < target)) ? 1.0f : 0.0f;
+        for (int i = 0; i < N; ++i) before += comes_before(x[i], first + i, xt, reach, target) ? 1.0f : 0.0f;
       }
     }
   }
@@ -353,10 +359,12 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
   const int full = v1 - (kBatch - 1) * kThreads;  // a whole batch starts below
   if (v < full) load(v);
   const bool given = target >= 0 && target < p.vocab;
-  const float xt = given ? L::get(x + target) : INFINITY;
+  float xt = given ? L::get(x + target) : INFINITY;
+  if (xt != xt) xt = -INFINITY;  // NaN ranks as -inf (the row's sums, and with them its results, are NaN then)
+  const float reach = xt == -INFINITY ? NAN : xt;
 
   Pass<T> pass;
-  if (at_head >= 0) pass.take(L::get(x + at_head), at_head, xt, target);
+  if (at_head >= 0) pass.take(L::get(x + at_head), at_head, xt, reach, target);
   while (v < full) {
     uint4 now[kBatch];
 #pragma unroll
@@ -364,13 +372,13 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
     const int at = head + v * N;
     v += stride;
     if (v < full) load(v);
-    pass.template take<kBatch>(now, at, kThreads, xt, target);
+    pass.template take<kBatch>(now, at, kThreads, xt, reach, target);
   }
   for (; v < v1; v += kThreads) {
     const uint4 one = __ldg(body + v);
-    pass.template take<1>(&one, head + v * N, 0, xt, target);
+    pass.template take<1>(&one, head + v * N, 0, xt, reach, target);
   }
-  if (at_tail >= 0) pass.take(L::get(x + at_tail), at_tail, xt, target);
+  if (at_tail >= 0) pass.take(L::get(x + at_tail), at_tail, xt, reach, target);
 
   Stats st = pass.stats();
   int before = (int)pass.before;
@@ -524,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
     if (bad_target) report_status(p.status, kStatusTokenRange, kWhereScore, target, row);
     if (p.logprobs) p.logprobs[row] = bad_target ? NAN : (given ? log_p(xt) : 0.0f);
     if (p.entropy) p.entropy[row] = none ? 0.0f : log_s - r.u / r.s;
-    if (p.ranks) p.ranks[row] = given ? before : -1;
+    if (p.ranks) p.ranks[row] = !given ? -1 : xt == -INFINITY ? before + target : before;
   }
   if (TOP) {
     // A key's place in the row: its place in its own list and the larger keys of the others.
