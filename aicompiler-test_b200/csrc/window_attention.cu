@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
       for (int i = 0; i < 2; ++i)
         qa[kk][half + 2 * i] = there ? *reinterpret_cast<const uint32_t *>(q + kk * 16 + 2 * tq + 8 * i) : 0u;
   }
-  bool poisoned = false;  // an infinity or NaN beside masked pairs
+  bool poisoned = false;  // an infinity or NaN that the products do not treat as slow_row does
   const float scale = p.scale * kLog2e;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
   float acc[D / 8][4];
@@ -280,11 +280,19 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
   }
   pdl_launch_dependents();
   cp_async_wait<0>();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float2 sum[2] = {};
+#pragma unroll
+    for (int dt = 0; dt < D / 8; ++dt) note_finite(sum[dt & 1], acc[dt][2 * half], acc[dt][2 * half + 1]);
+    const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    poisoned |= all != all && l_run[half] == l_run[half];
+  }
 
   // Join the warps: their states in shared memory, over the rings.
   float *w_acc = reinterpret_cast<float *>(smem);                                  // [warp][16][D]
   float2 *w_ml = reinterpret_cast<float2 *>(smem + C::kWarps * 16 * D * 4);        // [warp][16]
-  if (ROWS && __syncthreads_or(poisoned)) {  // the rows again, by plain loops; one state each
+  if (__syncthreads_or(poisoned)) {  // the rows again, by plain loops; one state each
     for (int r = warp; r < used; r += C::kWarps) {
       float mm, ll, o[(D + 31) / 32];
       slow_row<E, D>(p, seq, s, h, head_of(r), row_of(r), vis, v0, v1, mm, ll, o, lane);
@@ -296,7 +304,6 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
       }
     }
   } else {
-    if (!ROWS) __syncthreads();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = gq + 8 * half;
@@ -558,8 +565,18 @@ __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
   pdl_launch_dependents();
   cp_async_wait<0>();
 
+  bool lost = false;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float2 sum{};
+#pragma unroll
+    for (int dt = 0; dt < D / 8; ++dt) note_finite(sum, acc[dt][2 * half], acc[dt][2 * half + 1]);
+    const float all = sum.x + sum.y;
+    lost |= all != all && l_run[half] == l_run[half];
+  }
+
   const long long slots = (long long)p.sequences * p.max_rows * p.hq;
-  if (poisoned) {
+  if (poisoned || __any_sync(0xffffffffu, lost)) {
     for (int r = 0; r < 16; ++r) {
       const int m = m0 + warp * 16 + r;
       if (m >= total) break;

@@ -187,9 +187,17 @@ __device__ __forceinline__ float2 *partial_ml(const WindowAttentionParams &p, lo
   return reinterpret_cast<float2 *>(static_cast<float *>(p.workspace) + splits * slots * p.d) + split * slots + slot;
 }
 
+// Adds 0 for finite numbers, NaN for others.
+__device__ __forceinline__ void note_finite(float2 &sum, float a, float b) {
+  sum = __ffma2_rn(make_float2(a, b), make_float2(0.0f, 0.0f), sum);
+}
+
 // One tile row by plain loops over its own keys (a warp, lanes along D): used
 // when a step's values hold an infinity or NaN that some of the tile's rows do
-// not see, which 0 x value products would let through.
+// not see, which 0 x value products would let through; and when a result is not
+// finite although the row's sum is: an infinite value times a weight's low part
+// (decoding), or times a weight below the storage type's range (prompts), is
+// not what the weight in fp32 makes of it.
 template <typename E, int D>
 __device__ __noinline__ void slow_row(const WindowAttentionParams &p, const Sequence &seq, int s, int h, int head, int row,
                                       const Visible &vis, int v0, int v1, float &m, float &l, float (&o)[(D + 31) / 32],

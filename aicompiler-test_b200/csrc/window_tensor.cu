@@ -25,7 +25,8 @@
 //
 // Values that are infinite or NaN in a step that some row does not wholly see
 // would reach that row as 0 x inf: such a step marks the tile, and the tile's
-// rows are computed again by plain loops.
+// rows are computed again by plain loops. So are a warp's rows when one of
+// their results is not finite although its sum is (slow_row).
 //
 // Bound: the tensor pipe, at 81 to 90 cycles per product of 128 x 128 x 16 (88
 // would be 1675 TFLOP/s, a library product's, at 1.9 GHz), 32 of them per 128 keys of both tiles, beside a
@@ -473,26 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (t == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
       else asm volatile("bar.sync 2, 128;" ::: "memory");
       const long long slot = ((long long)s * p.max_rows + row) * p.hq + head;
-      if (!failed && marked[t] != 0) {
-        for (int i = 0; i < 32; ++i) {
-          const int mi = m0 + t * kTileRows + (warp & 3) * 32 + i;
-          if (mi >= total) break;
-          const int q_row = mi / g, q_head = h * g + mi % g;
-          float mm, ll, o[(D + 31) / 32];
-          slow_row<E, D>(p, seq, s, h, q_head, q_row, vis, v0, v1, mm, ll, o, lane);
-          const long long q_slot = ((long long)s * p.max_rows + q_row) * p.hq + q_head;
-#pragma unroll
-          for (int n = 0; n < D / 32; ++n) {
-            const int d = lane + 32 * n;
-            if (splits > 1)
-              partial_acc(p, slots, split, q_slot)[d] = o[n];
-            else
-              store1(p.out, (seq.start + q_row) * p.out_stride + (long long)q_head * D + d,
-                     ll > 0.0f || ll != ll ? o[n] / ll : 0.0f, E());
-          }
-          if (splits > 1 && lane == 0) *partial_ml(p, slots, splits, split, q_slot) = make_float2(mm, ll);
-        }
-      } else if (!failed) {
+      bool again = marked[t] != 0;  // by plain loops
+      if (!failed && !again) {
         const float l = (l_run[0].x + l_run[0].y) + (l_run[1].x + l_run[1].y);
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // no visible key: zeros
         // Q has been read: its place takes the results, 256-byte (D 64: 128-byte) pieces of each row.
@@ -511,6 +494,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         };
+        float2 finite{};
+        auto lost = [&] {
+          const float all = finite.x + finite.y;
+          return __any_sync(0xffffffffu, used && all != all && l == l) != 0;
+        };
         if (splits > 1) {
 #pragma unroll 1
           for (int part = 0; part < 2; ++part) {  // D / 2 fp32 columns fill a row's place
@@ -519,17 +507,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               float x[32];
               tmem_load32(o_at + part * (D / 2) + c, x);
 #pragma unroll
+              for (int i = 0; i < 32; i += 2) note_finite(finite, x[i], x[i + 1]);
+#pragma unroll
               for (int i = 0; i < 8; ++i)
                 *reinterpret_cast<float4 *>(own_rows + swizzled(r, c / 4 + i)) =
                     make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
             hand_out(static_cast<char *>(p.workspace), 4, part * D * 2);
           }
+          again = lost();
         } else {
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             float x[32];
             tmem_load32(o_at + c, x);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) note_finite(finite, x[i], x[i + 1]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               *reinterpret_cast<uint4 *>(own_rows + swizzled(r, c / 8 + i)) =
@@ -538,9 +531,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                              pack2(x[8 * i + 4] * inv, x[8 * i + 5] * inv, E()),
                              pack2(x[8 * i + 6] * inv, x[8 * i + 7] * inv, E()));
           }
-          hand_out(static_cast<char *>(p.out), 2, 0);
+          again = lost();
+          if (!again) hand_out(static_cast<char *>(p.out), 2, 0);  // the queries may lie there
         }
         if (used && splits > 1) *partial_ml(p, slots, splits, split, slot) = make_float2(m_run, l);
+      }
+      if (!failed && again) {
+        __syncwarp();
+        for (int i = 0; i < 32; ++i) {
+          const int mi = m0 + t * kTileRows + (warp & 3) * 32 + i;
+          if (mi >= total) break;
+          const int q_row = mi / g, q_head = h * g + mi % g;
+          float mm, ll, o[(D + 31) / 32];
+          slow_row<E, D>(p, seq, s, h, q_head, q_row, vis, v0, v1, mm, ll, o, lane);
+          const long long q_slot = ((long long)s * p.max_rows + q_row) * p.hq + q_head;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            const int d = lane + 32 * n;
+            if (splits > 1)
+              partial_acc(p, slots, split, q_slot)[d] = o[n];
+            else
+              store1(p.out, (seq.start + q_row) * p.out_stride + (long long)q_head * D + d,
+                     ll > 0.0f || ll != ll ? o[n] / ll : 0.0f, E());
+          }
+          if (splits > 1 && lane == 0) *partial_ml(p, slots, splits, split, q_slot) = make_float2(mm, ll);
+        }
       }
     }
   } else if (BOXES && warp < kMmaWarp) {
