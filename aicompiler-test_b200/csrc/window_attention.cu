@@ -87,13 +87,55 @@ struct DecodeCfg {
   static constexpr int smem(int rows) { return kSmem + (rows * D + 4 * kMaxCluster) * 4; }
 };
 
+// An infinite value times both parts of a weight is NaN where the low part is 0
+// or negative. A thread that has written a NaN although the row's sum is none
+// puts the sum of the values that are not finite in its place, looked for among
+// the keys once more: an infinity, or NaN. It finds its place anew: what the
+// kernel would have to keep for it slows its loop down (64 sequences 160 us for
+// 146, with the loop below inside the kernel).
+template <typename E, int D, bool ROWS>
+__device__ __noinline__ void infinite_values(const WindowAttentionParams &p, int tiles, int cluster) {
+  const int s = blockIdx.z, h = blockIdx.y / tiles, m0 = blockIdx.y % tiles * 16, splits = gridDim.x;
+  const int crank = blockIdx.x % cluster, outer = blockIdx.x / cluster, outers = splits / cluster;
+  const Sequence seq = load_sequence(p, s, false);
+  const int g = p.hq / p.hkv, used = min(16, seq.rows * g - m0);
+  auto row_of = [&](int r) { return ROWS ? (m0 + r) / g : 0; };
+  const Visible vis = visible_keys(p, seq.first + row_of(0), seq.first + row_of(used - 1));
+  const int chunk = ((vis.count + splits - 1) / splits + 15) / 16 * 16;
+  const int v0 = min(vis.count, outer * cluster * chunk), v1 = min(vis.count, v0 + cluster * chunk);
+  const int share = ((used * D + cluster - 1) / cluster + 3) & ~3;
+  const int e1 = min(used * D, (crank + 1) * share);
+  const long long slots = (long long)p.sequences * p.max_rows * p.hq;
+  for (int i = crank * share + (int)threadIdx.x * 4; i < e1; i += 128 * 4) {
+    const int r = i / D, d = i % D, row = row_of(r), head = h * g + m0 + r - row * g, at = seq.first + row;
+    float sum[4] = {};
+    for (int v = v0; v < v1; ++v) {
+      const int j = vis.key(v);
+      if (j > at || (at - j >= p.window && j >= p.sinks)) continue;
+      const KeyPlace k = find_key(p, seq.table, j);
+      if (k.page < 0 || k.page >= p.pool_pages) continue;
+      const E *x = static_cast<const E *>(p.v_pool) + (((long long)k.page * p.hkv + h) * p.page_size + k.offset) * D + d;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] += isfinite((float)x[c]) ? 0.0f : (float)x[c];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (sum[c] == 0.0f) continue;
+      if (outers > 1)
+        partial_acc(p, slots, outer, ((long long)s * p.max_rows + row) * p.hq + head)[d + c] = sum[c];
+      else
+        store1(p.out, (seq.start + row) * p.out_stride + (long long)head * D + d + c, sum[c], E());
+    }
+  }
+}
+
 // Grid (splits, Hkv x tiles, sequences), clusters of `cluster` CTAs along the
 // splits; outer = splits / cluster of them meet in the workspace. A tile is 16
 // of the (row, head of the KV head) pairs, heads fastest. ROWS: sequences may
 // have several rows, whose masks differ.
 template <typename E, int D, bool ROWS>
 __global__ void __launch_bounds__(128, kDecodePerSm)
-    window_decode_kernel(const WindowAttentionParams p, int tiles, int cluster) {
+    window_decode_kernel(const __grid_constant__ WindowAttentionParams p, int tiles, int cluster) {
   using C = DecodeCfg<D>;
   constexpr int S = C::kStages;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -171,7 +213,7 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
       for (int i = 0; i < 2; ++i)
         qa[kk][half + 2 * i] = there ? *reinterpret_cast<const uint32_t *>(q + kk * 16 + 2 * tq + 8 * i) : 0u;
   }
-  bool poisoned = false;  // an infinity or NaN that the products do not treat as slow_row does
+  bool poisoned = false;  // an infinity or NaN beside masked pairs
   const float scale = p.scale * kLog2e;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
   float acc[D / 8][4];
@@ -280,19 +322,11 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
   }
   pdl_launch_dependents();
   cp_async_wait<0>();
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float2 sum[2] = {};
-#pragma unroll
-    for (int dt = 0; dt < D / 8; ++dt) note_finite(sum[dt & 1], acc[dt][2 * half], acc[dt][2 * half + 1]);
-    const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-    poisoned |= all != all && l_run[half] == l_run[half];
-  }
 
   // Join the warps: their states in shared memory, over the rings.
   float *w_acc = reinterpret_cast<float *>(smem);                                  // [warp][16][D]
   float2 *w_ml = reinterpret_cast<float2 *>(smem + C::kWarps * 16 * D * 4);        // [warp][16]
-  if (__syncthreads_or(poisoned)) {  // the rows again, by plain loops; one state each
+  if (ROWS && __syncthreads_or(poisoned)) {  // the rows again, by plain loops; one state each
     for (int r = warp; r < used; r += C::kWarps) {
       float mm, ll, o[(D + 31) / 32];
       slow_row<E, D>(p, seq, s, h, head_of(r), row_of(r), vis, v0, v1, mm, ll, o, lane);
@@ -304,6 +338,7 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
       }
     }
   } else {
+    if (!ROWS) __syncthreads();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = gq + 8 * half;
@@ -323,8 +358,11 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
   const int crank = split % cluster, outer = split / cluster, outers = splits / cluster;
   const int share = ((used * D + cluster - 1) / cluster + 3) & ~3;
   const long long slots = (long long)p.sequences * p.max_rows * p.hq;
+  bool lost = false;  // a NaN of this thread's
   auto finish = [&](int i, const float4 &o, float m, float l) {  // elements i .. i + 3, of one row
     const int row = row_of(i / D), head = head_of(i / D);
+    const float all = (o.x + o.y) + (o.z + o.w);
+    lost |= all != all && l == l;
     if (outers > 1) {
       const long long slot = ((long long)s * p.max_rows + row) * p.hq + head;
       *reinterpret_cast<float4 *>(partial_acc(p, slots, outer, slot) + i % D) = o;
@@ -354,7 +392,10 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
     if (D / 4 < cluster && i % D == 0)
       for (int c = D / 4; c < cluster; ++c) store_cluster(&recv_ml[crank][r], c, m, l);
   }
-  if (cluster == 1) return;
+  if (cluster == 1) {
+    if (lost) infinite_values<E, D, ROWS>(p, tiles, cluster);
+    return;
+  }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int e0 = crank * share, e1 = min(used * D, e0 + share);
   for (int i = e0 + tid * 4; i < e1; i += 128 * 4) {
@@ -369,6 +410,7 @@ __global__ void __launch_bounds__(128, kDecodePerSm)
       if (c < cluster) join_part(recv_ml[c][r], *reinterpret_cast<const float4 *>(recv + c * share + i - e0), m, l, o);
     finish(i, o, m, l);
   }
+  if (lost) infinite_values<E, D, ROWS>(p, tiles, cluster);
 }
 
 // ---- prompts -------------------------------------------------------------------------------

@@ -194,10 +194,10 @@ __device__ __forceinline__ void note_finite(float2 &sum, float a, float b) {
 
 // One tile row by plain loops over its own keys (a warp, lanes along D): used
 // when a step's values hold an infinity or NaN that some of the tile's rows do
-// not see, which 0 x value products would let through; and when a result is not
-// finite although the row's sum is: an infinite value times a weight's low part
-// (decoding), or times a weight below the storage type's range (prompts), is
-// not what the weight in fp32 makes of it.
+// not see, which 0 x value products would let through; in prompts also when a
+// result is not finite although the row's sum is: an infinite value times a
+// weight below the storage type's range is NaN, where the weight in fp32 makes
+// it infinite.
 template <typename E, int D>
 __device__ __noinline__ void slow_row(const WindowAttentionParams &p, const Sequence &seq, int s, int h, int head, int row,
                                       const Visible &vis, int v0, int v1, float &m, float &l, float (&o)[(D + 31) / 32],

@@ -300,8 +300,9 @@ int tmc_k_paged_attention_f16_noalloc(const void *q, void *out, const void *k_po
  *            single-token decoding). A close bound: the launch is laid out for it
  * hq a multiple of hkv, d in {16, 32, 64, 128}, scale 0 for 1 / sqrt(d);
  * pointers 16-byte aligned. A row all of whose pages are missing becomes 0.
- * What a query does not see may hold anything; an infinite value that it sees
- * counts with the weight that fp32 gives it.
+ * What a query does not see may hold anything. An infinite value that it sees
+ * makes the result infinite (NaN with one of the other sign; NaN may stand for
+ * it too where its weight is 0 in fp32).
  * workspace: with tmc_k_window_attention_workspace_bytes(...) bytes a launch of
  * few rows over a wide window is split further; with fewer, or NULL, it is
  * split less and takes longer. Its contents need not be set, and nothing in it
