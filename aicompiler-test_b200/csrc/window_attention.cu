@@ -797,8 +797,7 @@ cudaError_t dispatch(const WindowAttentionParams &p, int num_sms, cudaStream_t s
 
 size_t window_attention_workspace_bytes(int sequences, int max_rows, int hq, int hkv, int d, long long window,
                                         long long sinks, int num_sms) {
-  if (sequences <= 0 || max_rows <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || d <= 0 || window <= 0 || sinks < 0)
-    return 0;
+  if (!can_plan(sequences, max_rows, hq, hkv) || d <= 0 || window <= 0 || sinks < 0) return 0;
   return partial_bytes(sequences, max_rows, hq, d,
                        most_splits(sequences, max_rows, hq, hkv, d,
                                    visible_bound(window, sinks, max_rows, 0x7fffffffll), num_sms));
@@ -806,20 +805,17 @@ size_t window_attention_workspace_bytes(int sequences, int max_rows, int hq, int
 
 int window_attention_launches(int sequences, int max_rows, int hq, int hkv, int d, long long window, long long sinks,
                               long long capacity, int num_sms) {
+  if (!can_plan(sequences, max_rows, hq, hkv)) return 1;
   const long long keys = visible_bound(window, sinks, max_rows, capacity);
   return make_plan(sequences, max_rows, hq, hkv, d, keys, num_sms).outer > 1 ? 2 : 1;
 }
 
 cudaError_t launch_window_attention(const WindowAttentionParams &p, bool bf16, int num_sms, cudaStream_t stream,
                                     bool pdl) {
-  if (p.sequences <= 0 || p.sequences > 65535 || p.rows < 0 || p.max_rows <= 0 || p.hkv <= 0 || p.hq <= 0 ||
-      p.hq % p.hkv != 0 || p.page_size <= 0 || p.pool_pages <= 0 || p.table_stride <= 0 || p.capacity <= 0 ||
+  if (!can_plan(p.sequences, p.max_rows, p.hq, p.hkv) || p.rows < 0 || p.page_size <= 0 || p.pool_pages <= 0 || p.table_stride <= 0 || p.capacity <= 0 ||
       p.window <= 0 || p.sinks < 0 || p.q_stride % 8 != 0 || p.out_stride % 8 != 0)
     return cudaErrorInvalidValue;
-  const long long g = p.hq / p.hkv;
-  if ((long long)p.hkv * ((g + 15) / 16) > 65535 || p.hq > 65535 || (long long)p.max_rows * g > (1ll << 30) / kMaxOuter ||
-      (long long)p.sequences * p.max_rows > (1ll << 32) / p.hq ||
-      (long long)p.pool_pages * p.hkv > (1ll << 32) / p.page_size - 1)  // pool rows are counted in 32 bits
+  if ((long long)p.pool_pages * p.hkv > (1ll << 32) / p.page_size - 1)  // pool rows are counted in 32 bits
     return cudaErrorInvalidValue;
   WindowAttentionParams q = p;
   q.page_shift = -1;

@@ -28,11 +28,21 @@ struct Plan {
   int outer;    // splits that join through the workspace
 };
 
+// Whether a call of this size can be launched: grids and tile rows within
+// their types.
+inline bool can_plan(int sequences, int max_rows, int hq, int hkv) {
+  if (sequences <= 0 || sequences > 65535 || max_rows <= 0 || hkv <= 0 || hq <= 0 || hq > 65535 || hq % hkv != 0)
+    return false;
+  const long long g = hq / hkv;
+  return hkv * ((g + 15) / 16) <= 65535 && max_rows * g <= (1ll << 30) / kMaxOuter &&
+         (long long)sequences * max_rows <= (1ll << 32) / hq;
+}
+
 inline size_t partial_bytes(int sequences, int max_rows, int hq, int d, int outer) {
   return outer <= 1 ? 0 : (size_t)outer * sequences * max_rows * hq * (d + 2) * sizeof(float);
 }
 
-// keys: the most keys a row can see.
+// keys: the most keys a row can see. For calls that can_plan accepts.
 inline Plan make_plan(int sequences, int max_rows, int hq, int hkv, int d, long long keys, int num_sms) {
   const int g = hq / hkv;
   const long long tile_rows = (long long)max_rows * g, few_tiles = (tile_rows + 15) / 16 * hkv;  // tiles of decoding

@@ -78,3 +78,10 @@ def test_a_shorter_capacity_can_mean_more_splits(lib):
     shape = (1, 1000, 8, 8, 64)
     assert [plan(lib, shape, 128 * steps)["outer"] for steps in (4, 5)] == [4, 3]
     assert lib.most_splits(*shape, 640, SMS) == 4
+
+
+@pytest.mark.parametrize("sequences,max_rows,hq,hkv,d", [
+    (1, 2 ** 30, 1024, 1, 64), (1, 2 ** 31 - 1, 512, 1, 128), (2 ** 31 - 1, 1, 32, 8, 128), (65536, 1, 4, 1, 64),
+    (1, 1, 2 ** 31 - 1, 1, 64), (1, 2 ** 26, 1, 1, 32), (60000, 60000, 65535, 1, 16), (1, 1, 65535 * 17, 65535, 64)])
+def test_calls_that_cannot_be_launched_need_no_workspace(sequences, max_rows, hq, hkv, d):
+    assert tmc_cuda.lib.tmc_k_window_attention_workspace_bytes(sequences, max_rows, hq, hkv, d, 1024, 0) == 0
