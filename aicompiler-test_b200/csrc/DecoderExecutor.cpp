@@ -925,6 +925,10 @@ int DecoderExecutor::kernelsPerStep(int rows) const {
   return cfg_.layers * perLayer + head + (tp && !peersAttached_ ? 1 : 0);  // + argmax finalize after the collective
 }
 
+double DecoderExecutor::seenPositions(double length) const {
+  return window_ > 0 ? std::min(length, (double)window_ + sinks_) : length;
+}
+
 double DecoderExecutor::stepAlgorithmicBytes(int rows, const std::vector<int> &ctx) const {
   const double H = cfg_.hidden, D = cfg_.headDim;
   double w = 0.0;
@@ -932,10 +936,7 @@ double DecoderExecutor::stepAlgorithmicBytes(int rows, const std::vector<int> &c
   w *= cfg_.layers;
   w += (double)vL_ * H + H;  // LM head + final norm
   double bytes = 2.0 * w + 2.0 * rows * H;  // weights + embedding rows
-  for (int c : ctx) {  // K and V reads
-    const double seen = window_ > 0 ? std::min<double>(c, (double)window_ + sinks_) : c;
-    bytes += 2.0 * 2.0 * hkvL_ * D * seen * cfg_.layers;
-  }
+  for (int c : ctx) bytes += 2.0 * 2.0 * hkvL_ * D * seenPositions(c) * cfg_.layers;  // K and V reads
   bytes += 2.0 * 2.0 * hkvL_ * D * rows * cfg_.layers;                // K and V appends
   return bytes;
 }
@@ -1357,7 +1358,7 @@ std::string DecoderExecutor::profileKernel(int kind, int R, int rounds, double *
       break;
     case kKernelAttention: {
       double ctx = 0.0;
-      for (int r = 0; r < R; ++r) ctx += lastPositions_[r] + 1.0;
+      for (int r = 0; r < R; ++r) ctx += seenPositions(lastPositions_[r] + 1.0);
       bytes = 2.0 * 2.0 * hkvL_ * D * ctx + 2.0 * 2.0 * R * hqL_ * D;
       break;
     }

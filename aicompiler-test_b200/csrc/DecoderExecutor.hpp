@@ -220,6 +220,8 @@ class DecoderExecutor {
 
  private:
   std::string ensureSpill(std::size_t bytes, int npages);
+  // Positions of a sequence of that length that its newest query sees.
+  double seenPositions(double length) const;
   std::string ensurePoolPointers();
   std::string ensurePageLists(std::size_t count);
   std::string copyPages(const std::vector<KVPageCopy> &copies);

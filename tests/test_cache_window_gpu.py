@@ -1,6 +1,5 @@
 """Windows of the decoder beside its other calls."""
 
-import numpy as np
 import pytest
 
 from test_cache_decoder_gpu import Model
@@ -13,3 +12,16 @@ def test_kernels_of_any_number_of_rows(rt):
     off = [m.dec.kernels_per_step(r) for r in (0, 1, 64)]
     m.dec.set_window(48, 4)
     assert [m.dec.kernels_per_step(r) for r in (0, 1, 64)] == off  # these need no second kernel
+
+
+def test_a_windowed_attentions_bytes_are_those_that_it_reads(rt):
+    m = Model(rt)  # 2 KV heads and 8 heads of 64
+    prompt = m.tokens(100)
+    m.dec.prefill(prompt)
+    m.dec.decode([1])
+    queries = 2 * 2 * 8 * 64  # Q in, results out
+    per_position = 2 * 2 * 2 * 64
+    assert m.dec.profile_kernel(1, 1, 2)[1] == 101 * per_position + queries
+    for window, sinks, seen in ((20, 3, 23), (200, 3, 101), (99, 1, 100), (100, 30, 101)):
+        m.dec.set_window(window, sinks)
+        assert m.dec.profile_kernel(1, 1, 2)[1] == seen * per_position + queries
