@@ -1376,6 +1376,7 @@ std::string DecoderExecutor::profileKernel(int kind, int R, int rounds, double *
       break;
   }
   const int perRound = kind == kKernelLMHead ? 1 : cfg_.layers;
+  if (kind == kKernelLMHead) logitRows_ = 0;  // its logits are of no step
   cudaStream_t s = rt_.stream();
   auto sync = rt_.synchronize();
   if (!sync.empty()) return sync;

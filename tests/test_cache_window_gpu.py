@@ -25,3 +25,19 @@ def test_a_windowed_attentions_bytes_are_those_that_it_reads(rt):
     for window, sinks, seen in ((20, 3, 23), (200, 3, 101), (99, 1, 100), (100, 30, 101)):
         m.dec.set_window(window, sinks)
         assert m.dec.profile_kernel(1, 1, 2)[1] == seen * per_position + queries
+
+
+def test_logits_of_a_profile_are_not_scored(rt):
+    import tmc_cuda
+    m = Model(rt)
+    m.dec.prefill(m.tokens(20))
+    m.dec.decode([1])
+    first = m.dec.token_logprobs(1)["logprobs"]
+    m.dec.profile_kernel(1, 1, 2)
+    assert m.dec.token_logprobs(1)["logprobs"] == first  # attention leaves the logits
+    m.dec.profile_kernel(0, 1, 2)
+    m.dec.profile_kernel(5, 1, 2)
+    with pytest.raises(tmc_cuda.TmcError, match="last step"):
+        m.dec.token_logprobs(1)
+    m.dec.decode([2])
+    assert m.dec.token_logprobs(1)["ranks"][0] == 0
