@@ -1613,6 +1613,7 @@ std::string DecoderExecutor::tokenScores(const std::int32_t *targets, int rows, 
 
 std::string DecoderExecutor::setWindow(int window, int sinks) {
   if (window < 0 || sinks < 0) return "window and sinks must not be negative.";
+  if (window >= cfg_.capacity) window = 0;  // hides nothing: by the kernels without a window
   const int D = cfg_.headDim;
   if (window > 0 && D != 16 && D != 32 && D != 64 && D != 128)
     return "window attention needs a head dimension of 16, 32, 64 or 128.";
@@ -1633,9 +1634,9 @@ std::string DecoderExecutor::setWindow(int window, int sinks) {
     std::size_t bytes = 0;
     for (int r = 1; r <= M; ++r) {
       bytes = std::max(bytes, tmc::window_attention_workspace_bytes(r, 1, hqL_, hkvL_, cfg_.headDim,
-                                                                    std::min(window, cfg_.capacity), sinks, numSms_));
-      bytes = std::max(bytes, tmc::window_attention_workspace_bytes(1, r, hqL_, hkvL_, cfg_.headDim,
-                                                                    std::min(window, cfg_.capacity), sinks, numSms_));
+                                                                    window, sinks, numSms_));
+      bytes = std::max(bytes, tmc::window_attention_workspace_bytes(1, r, hqL_, hkvL_, cfg_.headDim, window, sinks,
+                                                                    numSms_));
     }
     if (bytes > 0 && (!windowWorkspace_ || windowWorkspace_->byteCount() < bytes)) {
       auto r = rt_.createBuffer(bytes / 4 + 1, nullptr, ElementType::Float32);

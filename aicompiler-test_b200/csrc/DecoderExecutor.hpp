@@ -195,7 +195,8 @@ class DecoderExecutor {
   // (the last position has none: log probability 0, rank -1).
   std::string score(int slot, const std::int32_t *tokens, int count, const TokenScores &out, std::int32_t *nextToken);
   // Attend only to the newest `window` positions (the query's own included) and
-  // to the first `sinks`; window 0: to all, by the kernels without a window.
+  // to the first `sinks`; window 0, or one that covers the capacity: to all, by
+  // the kernels without a window.
   std::string setWindow(int window, int sinks);
   std::vector<std::int32_t> blockTable(int slot) const;
   // [localKVHeads, length, headDim] logical values (reference readKeyPrefix).

@@ -571,9 +571,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kThreads)
       acc[dt][3] *= rescale[1];
     }
     // P is rounded once to the storage type (its largest entry is at most 1;
-    // the sum l is taken before the rounding): each output then carries
-    // independent errors of half a step per key, which together stay below
-    // the rounding of the output itself.
+    // the sum l is taken before the rounding), as in window_tensor.cu: an output
+    // is off by 2^-11 (fp16) or 2^-8 (bf16) of sum p |v| at most, beside its own
+    // rounding.
 #pragma unroll
     for (int kk = 0; kk < BN / 16; ++kk) {
       uint32_t pa[4];

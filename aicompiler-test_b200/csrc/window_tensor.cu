@@ -19,9 +19,13 @@
 // floating-point numbers lose nothing below that, and O is not rescaled in most
 // steps.
 //
-// P is rounded once to the storage type; the row sum l is taken before that.
-// Each output then carries independent errors of half a step per key, which
-// together stay below the rounding of the output itself.
+// P is rounded once to the storage type; the row sum l is taken before that. An
+// output is then off by 2^-11 (fp16) or 2^-8 (bf16) of sum p |v| at most: in the
+// mean about as much again as its own rounding (four bf16 prompts: 0.0023 of the results' size against
+// 64 bits, 0.0016 with weights in fp32; a chunk in fp16 0.00028 and 0.00021).
+// A second part of P, as in decoding, is half as many products again, where
+// products are the bound, and for heads of 128 has no place: one S, two P and two
+// O fill tensor memory.
 //
 // Values that are infinite or NaN in a step that some row does not wholly see
 // would reach that row as 0 x inf: such a step marks the tile, and the tile's

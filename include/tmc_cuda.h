@@ -302,7 +302,10 @@ int tmc_k_paged_attention_f16_noalloc(const void *q, void *out, const void *k_po
  * pointers 16-byte aligned. A row all of whose pages are missing becomes 0.
  * What a query does not see may hold anything. An infinite value that it sees
  * makes the result infinite (NaN with one of the other sign; NaN may stand for
- * it too where its weight is 0 in fp32).
+ * it too where its weight is 0 in fp32). Scores, sums and results are held in
+ * fp32. The softmax weights p of prompts (more than a few rows) are rounded once
+ * to the storage type, which moves a result by 2^-11 (fp16) or 2^-8 (bf16) of
+ * sum p |v| at most; those of single and few rows keep twice the bits.
  * workspace: with tmc_k_window_attention_workspace_bytes(...) bytes a launch of
  * few rows over a wide window is split further; with fewer, or NULL, it is
  * split less and takes longer. Its contents need not be set, and nothing in it
@@ -617,9 +620,11 @@ int tmc_decoder_attach_peers(tmc_decoder *dec, const uint8_t *handles, size_t nb
 int tmc_decoder_attach_local_peers(tmc_decoder *dec, tmc_decoder *const *ranks, int world, int rank);
 /* Sliding window: from now on the queries of this decoder attend to the newest
  * `window` positions (their own included) and to the first `sinks` positions of
- * their sequence (tmc_k_window_attention's rule). 0: all positions, the state
- * after creation. Positions keep their cache rows; to free rows, and to go on
- * beyond the capacity, drop positions with tmc_decoder_compact. */
+ * their sequence (tmc_k_window_attention's rule, and its rounding of a prompt's
+ * weights). 0: all positions, the state after creation; a window that covers the
+ * capacity is the same. Positions keep their cache rows; to free rows, and to go
+ * on beyond the capacity, drop positions with tmc_decoder_compact. Under tensor
+ * parallelism every rank sets the same window, and forks and compacts alike. */
 int tmc_decoder_set_window(tmc_decoder *dec, int window, int sinks);
 
 /* Make every slot of `slots` (empty, distinct) a fork of `slot`: the pages that

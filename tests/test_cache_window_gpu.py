@@ -1,5 +1,6 @@
 """Windows of the decoder beside its other calls."""
 
+import numpy as np
 import pytest
 
 from test_cache_decoder_gpu import Model
@@ -41,3 +42,18 @@ def test_logits_of_a_profile_are_not_scored(rt):
         m.dec.token_logprobs(1)
     m.dec.decode([2])
     assert m.dec.token_logprobs(1)["ranks"][0] == 0
+
+
+@pytest.mark.parametrize("window,sinks", [(512, 0), (600, 7), (2 ** 31 - 1, 0)])
+@pytest.mark.parametrize("head_dim,heads,kv_heads", [(64, 8, 2), (32, 8, 2), (128, 4, 4)])
+def test_a_window_that_hides_nothing_is_none(rt, window, sinks, head_dim, heads, kv_heads):
+    m = Model(rt, heads, kv_heads, head_dim)  # a capacity of 512
+    other = m.make()
+    other.set_window(window, sinks)
+    for x, y in zip(m.dec.prefill(m.tokens(150)), other.prefill(m.tokens(150))):
+        assert np.array_equal(x, y)
+    for x, y in zip(m.dec.decode([5]), other.decode([5])):
+        assert np.array_equal(x, y)
+    for layer in range(2):
+        for x, y in zip(m.dec.read_kv(layer), other.read_kv(layer)):
+            assert np.array_equal(x, y)
