@@ -38,10 +38,9 @@ def _library():
     return tmc_cuda, tmc_cuda.Runtime(0)
 
 
-@functools.lru_cache(maxsize=None)
 def _workspace(nbytes):
-    """A workspace of this size, kept for later calls of the same plan."""
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+    """A call's own workspace, of the current stream: calls may overlap on the GPU."""
+    return torch.empty(nbytes, dtype=torch.uint8, device="cuda") if nbytes else None
 
 
 def _stream():
