@@ -790,6 +790,8 @@ std::string DecoderExecutor::compactSlot(int slot, const std::int32_t *keep, int
     if (keep[i] < 0 || (std::size_t)keep[i] >= length || (i > 0 && keep[i] <= keep[i - 1]))
       return "compact: kept positions must ascend within the committed length.";
   if (cfg_.headDim % 8 != 0) return "compact: head dimension must be a multiple of 8.";
+  const auto old = st.pageTable();
+  if (old.size() * P < length) return "compact: KV page missing for a committed position.";
   std::size_t same = 0;  // rows that stay where they are
   while (same < (std::size_t)count && keep[same] == (std::int32_t)same) ++same;
   if (same == (std::size_t)count) return rollbackLength(slot, count);
@@ -807,7 +809,6 @@ std::string DecoderExecutor::compactSlot(int slot, const std::int32_t *keep, int
     fresh.push_back(page);
   }
   // Device lists: the sequence's pages, the new ones (by new position), the kept positions.
-  const auto old = st.pageTable();
   std::vector<std::int32_t> lists(old);
   lists.insert(lists.end(), old.begin(), old.begin() + (std::ptrdiff_t)lead);
   lists.insert(lists.end(), fresh.begin(), fresh.end());

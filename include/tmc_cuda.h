@@ -629,7 +629,9 @@ int tmc_decoder_set_window(tmc_decoder *dec, int window, int sinks);
 
 /* Make every slot of `slots` (empty, distinct) a fork of `slot`: the pages that
  * its committed positions fill are shared until their last owner lets them go,
- * a partly filled last page is copied. The forks then go their own ways. */
+ * a partly filled last page is copied. The forks then go their own ways: none
+ * writes into a page that another holds. Needs a page for every committed
+ * position, as does compaction. */
 int tmc_decoder_fork(tmc_decoder *dec, int slot, const int32_t *slots, int count);
 
 /* Keep only the committed positions keep[0 .. count) (ascending) of a sequence:

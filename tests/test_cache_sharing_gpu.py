@@ -44,3 +44,17 @@ def test_committed_positions_without_pages_cannot_be_forked(rt):
     with pytest.raises(tmc_cuda.TmcError, match="every committed position"):
         m.dec.fork(0, [1, 2])
     assert m.dec.pool_stats()["used"] == 2 and m.dec.length(1) == m.dec.length(2) == 0
+
+
+def test_committed_positions_without_pages_cannot_be_compacted(rt):
+    import tmc_cuda
+    m = Model(rt)
+    m.dec.prefill(m.tokens(20))
+    m.dec.commit(0, 100)  # two pages of 16 are there
+    for keep in (list(range(40)) + [99], [3, 99], list(range(90))):
+        with pytest.raises(tmc_cuda.TmcError, match="missing"):
+            m.dec.compact(0, keep)
+        assert m.dec.length(0) == 100 and m.dec.pool_stats()["used"] == 2
+    m.dec.commit(0, 20)
+    m.dec.compact(0, [0, 19])
+    assert m.dec.length(0) == 2
