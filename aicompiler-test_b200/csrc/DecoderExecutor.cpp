@@ -1670,8 +1670,8 @@ std::string DecoderExecutor::runPrefill(int slot, const std::int32_t *tokens, in
   // Chunks of maxRows rows (the reference's prefillChunked,
   // DecoderLLMExecutor.cpp:982-1034), queued back to back: each chunk's inputs
   // come from its own pinned staging block, so the host never waits between
-  // chunks; one synchronisation at the end (per chunk only when logits are
-  // copied to pageable host memory).
+  // chunks; one synchronisation at the end (per chunk only when logits or scores
+  // are copied to pageable host memory).
   const int M = cfg_.maxRows;
   logitRows_ = 0;
   std::vector<std::int32_t> pos(M), trow(M, slot);

@@ -25,7 +25,7 @@
 // Bound: many rows by issue slots (11.5 instructions a logit of 16 bits, of
 // which two for the exponential; 1500 rows of 50021 bf16 38 us, 3.9 TB/s, with
 // the last of two and a half rounds of CTAs part empty); one row of 128256 fp32
-// 7.9 us, by the chain of launch, reads, candidates and the cluster's joins.
+// 8.1 us, by the chain of launch, reads, candidates and the cluster's joins.
 #include "logprobs.cuh"
 
 #include <cuda_bf16.h>

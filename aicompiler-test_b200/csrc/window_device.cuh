@@ -121,9 +121,9 @@ __device__ __forceinline__ Sequence load_sequence(const WindowAttentionParams &p
 
 // A prompt CTA's place: grid.x counts KV heads fastest, then sequences, splits
 // and, last rows first, tiles. The last rows see the most keys: what takes
-// longest starts first, over all heads and sequences (heads slower than tiles:
-// 4096 rows of 32 heads 189 us instead of 161, 2048 rows of heads of 32 93 us
-// instead of 65).
+// longest starts first, over all heads and sequences. (Heads slower than tiles,
+// by the kernels of the time: 4096 rows of 32 heads 189 us instead of 161, which
+// take 137 today, 152 back to back; 2048 rows of heads of 32 93 us instead of 65.)
 struct PromptPlace {
   int head, seq, split, tile;
   bool first;  // one CTA of each sequence

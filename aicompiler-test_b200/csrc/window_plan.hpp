@@ -18,7 +18,7 @@ constexpr int kMaxOuter = 32;  // splits that meet through the workspace
 // has less to set up, but reads the keys for every 16 rows. 32 heads, 8 KV heads
 // of 128: 2 rows over 1000 keys 7.7 us (as prompts 13.9), 16 rows 10.7 (14.5), 32
 // rows (8.2 million) 14.8 (14.7), 64 rows (16 million) 20.0 (17.1); 64 sequences
-// of 4 rows over 1000 to 2000 keys 100 us (131), 16 heads of 64 of their own 92 (211).
+// of 4 rows over 1000 to 2000 keys 94 us (131), 16 heads of 64 of their own 86 (211).
 constexpr long long kFewElements = 12500000;
 
 struct Plan {

@@ -788,9 +788,10 @@ cudaError_t launch(const WindowAttentionParams &p, int pairs, int splits, cudaSt
 
 template <typename E, int D>
 cudaError_t dispatch(const WindowAttentionParams &p, int pairs, int splits, cudaStream_t stream, bool pdl) {
-  // Boxes of 16 positions where pages are whole numbers of them, else of 8 (4096
-  // rows, pages of 24: 165 us, by copies 209; pages of 16: 158, by boxes of 16
-  // 144). Pool rows are 32-bit coordinates.
+  // Boxes of 16 positions where pages are whole numbers of them, else of 8. 4096
+  // rows of 32 heads of 128: pages of 24 168 us, by copies 209; pages of 16 150, by
+  // boxes of 8 165. 2 x 4096 rows of 16 heads of 64, pages of 24: 131, by copies
+  // 165. Pool rows are 32-bit coordinates.
   if ((long long)p.pool_pages * p.hkv <= 0x7fffffffll / p.page_size) {
     if (p.page_size % 16 == 0) return launch<E, D, 16>(p, pairs, splits, stream, pdl);
     if (p.page_size % 8 == 0) return launch<E, D, 8>(p, pairs, splits, stream, pdl);
